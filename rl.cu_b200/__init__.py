@@ -1,4 +1,5 @@
-"""ctypes binding of ``librlcu_b200.so`` (the C ABI declared in ``include/rlcu_adamw.h``).
+"""ctypes binding of ``librlcu_b200.so`` (the C ABI declared in ``include/rlcu_adamw.h``,
+``include/rlcu_losses.h`` and ``include/rlcu_act8.h``).
 
 The directory name contains a dot, so it cannot be imported by name; load it with
 ``importlib`` under the module name ``rlcu_b200`` (``load_package()`` in
@@ -27,7 +28,13 @@ TENSOR_NORM_ONLY, TENSOR_GRAD_ZERO = 1, 2
 STEP_ROUND_CLIP_FP16, STEP_DEVICE_BIAS_CORRECTION, STEP_ZERO_GRADS, STEP_BULK_COPY, STEP_DIRECT = 1, 2, 4, 8, 16
 STAT_PARTIAL, STAT_ACCUMULATE = 1, 2
 
-# every symbol include/rlcu_adamw.h declares
+KL_K1, KL_K2, KL_K3 = 1, 2, 3
+PREF_SIGMOID, PREF_HINGE, PREF_IPO = 0, 1, 2
+LOSS_ACCUMULATE = 1
+ACT8_BLOCK = 128
+ACT8_ACCUMULATE = 1
+
+# every symbol the headers under include/ declare
 EXPORTS = [
     "rlcu_abi_version", "rlcu_last_error", "rlcu_adamw_fp16_master", "rlcu_adamw_fp16",
     "rlcu_adamw_bf16_master", "rlcu_adamw_bf16", "rlcu_adamw_fp32", "rlcu_half_to_float", "rlcu_tensor_list_create",
@@ -37,6 +44,9 @@ EXPORTS = [
     "rlcu_zero1_make_plan", "rlcu_zero1_plan_pieces", "rlcu_zero1_unique_id", "rlcu_zero1_create",
     "rlcu_zero1_step", "rlcu_zero1_poll_error", "rlcu_zero1_check", "rlcu_zero1_destroy",
     "rlcu_checkpoint_save", "rlcu_checkpoint_peek", "rlcu_checkpoint_load",
+    "rlcu_token_logprob", "rlcu_token_logprob_grad", "rlcu_policy_loss", "rlcu_policy_loss_logp", "rlcu_preference_loss",
+    "rlcu_act8_blocks", "rlcu_act8_store", "rlcu_act8_load", "rlcu_act8_rmsnorm", "rlcu_act8_rmsnorm_grad_workspace",
+    "rlcu_act8_rmsnorm_grad",
 ]
 UNIQUE_ID_BYTES = 128
 PHASE_REDUCE_SCATTER, PHASE_STATISTICS, PHASE_UPDATE, PHASE_ALL_GATHER = 1, 2, 4, 8
@@ -103,6 +113,32 @@ class CheckpointInfo(C.Structure):
                 ("world", C.c_int32), ("has_master", C.c_uint32), ("reserved", C.c_uint32)]
 
 
+class PolicyHParams(C.Structure):
+    """``rlcu_policy_hparams``."""
+    _fields_ = [("clip_low", C.c_float), ("clip_high", C.c_float), ("dual_clip", C.c_float),
+                ("kl_coef", C.c_float), ("kl_kind", C.c_uint32)]
+
+
+class PolicyStat(C.Structure):
+    """``rlcu_policy_stat`` (32 bytes, device memory)."""
+    _fields_ = [("loss", C.c_float), ("policy", C.c_float), ("kl", C.c_float), ("weight", C.c_float),
+                ("tokens", C.c_uint32), ("clipped", C.c_uint32), ("ratio_max", C.c_float), ("reserved", C.c_uint32)]
+
+
+class PreferenceHParams(C.Structure):
+    """``rlcu_preference_hparams``."""
+    _fields_ = [("beta", C.c_float), ("margin", C.c_float), ("label_smoothing", C.c_float),
+                ("kind", C.c_uint32), ("length_mean", C.c_uint32)]
+
+
+class PreferenceStat(C.Structure):
+    """``rlcu_preference_stat`` (32 bytes, device memory)."""
+    _fields_ = [("loss", C.c_float), ("margin", C.c_float), ("pairs", C.c_uint32), ("correct", C.c_uint32),
+                ("reserved", C.c_uint32 * 4)]
+
+
+assert C.sizeof(PolicyHParams) == 20 and C.sizeof(PolicyStat) == 32
+assert C.sizeof(PreferenceHParams) == 20 and C.sizeof(PreferenceStat) == 32
 assert C.sizeof(TensorDesc) == 64 and C.sizeof(Stat) == 64 and C.sizeof(ScalerState) == 32
 assert C.sizeof(CheckpointInfo) == 40
 assert C.sizeof(Zero1Segment) == 16 and C.sizeof(Zero1Plan) == 48
@@ -164,6 +200,20 @@ def lib() -> C.CDLL:
     L.rlcu_checkpoint_load.argtypes = [C.c_char_p, vp, vp, vp, vp, u64, vp]
     L.rlcu_bias_correction.argtypes = [f, C.c_int]
     L.rlcu_bias_correction.restype = f
+    logits = [vp, u32, u64, u64, u64, f, vp]          # data, dtype, rows, vocab, row stride, inv_temperature, targets
+    L.rlcu_token_logprob.argtypes = logits + [vp, vp, vp]
+    L.rlcu_token_logprob_grad.argtypes = logits + [vp, vp, vp, vp, u64, vp]
+    L.rlcu_policy_loss.argtypes = logits + [vp, vp, vp, vp, vp, vp, vp, vp, u64, vp, u32, vp]
+    L.rlcu_policy_loss_logp.argtypes = [vp, u64, vp, vp, vp, vp, vp, vp, vp, u32, vp]
+    L.rlcu_preference_loss.argtypes = [vp, u64, vp, vp, vp, u64, vp, vp, vp, vp, vp, u32, vp]
+    L.rlcu_act8_blocks.argtypes = [u64]
+    L.rlcu_act8_blocks.restype = u64
+    L.rlcu_act8_store.argtypes = [vp, u32, u64, u64, u64, vp, u64, vp, vp]
+    L.rlcu_act8_load.argtypes = [vp, u64, vp, u64, u64, vp, u32, u64, vp]
+    L.rlcu_act8_rmsnorm.argtypes = [vp, u64, vp, u64, u64, vp, u32, f, vp, u32, u64, vp, vp]
+    L.rlcu_act8_rmsnorm_grad_workspace.argtypes = [u64, u64]
+    L.rlcu_act8_rmsnorm_grad_workspace.restype = u64
+    L.rlcu_act8_rmsnorm_grad.argtypes = [vp, u64, vp, u64, u64, vp, u32, f, vp, u64, vp, u64, vp, u64, u32, vp, vp, u64, u32, vp]
     _lib = L
     return L
 
@@ -361,3 +411,90 @@ def checkpoint_load(path, m_ptr, v_ptr, master_ptr, capacity_elems, stream=None)
     check(lib().rlcu_checkpoint_load(os.fsencode(path), C.addressof(info), m_ptr, v_ptr, master_ptr,
                                      capacity_elems, stream))
     return info
+
+
+# ---------------------------------------------------------------------------
+# losses (include/rlcu_losses.h)
+# ---------------------------------------------------------------------------
+
+def token_logprob(logits_ptr, dtype, rows, vocab, targets_ptr, logp_ptr, lse=None, row_stride=0, inv_temperature=1.0,
+                  stream=None):
+    """Log-probabilities of the targets under ``rows`` rows of logits, and (``lse``) the rows' log-sum-exp."""
+    check(lib().rlcu_token_logprob(logits_ptr, dtype, rows, vocab, row_stride, inv_temperature, targets_ptr, logp_ptr,
+                                   lse, stream))
+
+
+def token_logprob_grad(logits_ptr, dtype, rows, vocab, targets_ptr, lse_ptr, coef_ptr, grad_ptr, row_stride=0,
+                       grad_stride=0, inv_temperature=1.0, scaler=None, stream=None):
+    """Gradient of the logits for ``coef`` = dloss/dlogp, times the loss scale of ``scaler``."""
+    check(lib().rlcu_token_logprob_grad(logits_ptr, dtype, rows, vocab, row_stride, inv_temperature, targets_ptr, lse_ptr,
+                                        coef_ptr, scaler, grad_ptr, grad_stride, stream))
+
+
+def policy_hparams(clip_low=0.2, clip_high=0.2, dual_clip=0.0, kl_coef=0.0, kl_kind=KL_K3) -> PolicyHParams:
+    return PolicyHParams(clip_low, clip_high, dual_clip, kl_coef, kl_kind)
+
+
+def policy_loss(logits_ptr, dtype, rows, vocab, targets_ptr, advantage_ptr, weight_ptr, hp: PolicyHParams, logp_ptr, grad_ptr,
+                stat_ptr, old_logp=None, ref_logp=None, row_stride=0, grad_stride=0, inv_temperature=1.0, scaler=None,
+                flags=0, stream=None):
+    """Clipped policy loss of a block of logits with its gradient (``grad_ptr`` None: the loss alone)."""
+    check(lib().rlcu_policy_loss(logits_ptr, dtype, rows, vocab, row_stride, inv_temperature, targets_ptr, old_logp, ref_logp,
+                                 advantage_ptr, weight_ptr, C.addressof(hp), scaler, logp_ptr, grad_ptr, grad_stride,
+                                 stat_ptr, flags, stream))
+
+
+def policy_loss_logp(logp_ptr, tokens, advantage_ptr, weight_ptr, hp: PolicyHParams, stat_ptr, coef=None, old_logp=None,
+                     ref_logp=None, flags=0, stream=None):
+    """Clipped policy loss of log-probabilities that are there already; ``coef`` receives dloss/dlogp."""
+    check(lib().rlcu_policy_loss_logp(logp_ptr, tokens, old_logp, ref_logp, advantage_ptr, weight_ptr, C.addressof(hp), coef,
+                                      stat_ptr, flags, stream))
+
+
+def preference_hparams(beta, margin=0.0, label_smoothing=0.0, kind=PREF_SIGMOID, length_mean=False) -> PreferenceHParams:
+    return PreferenceHParams(beta, margin, label_smoothing, kind, 1 if length_mean else 0)
+
+
+def preference_loss(logp_ptr, tokens, offsets_ptr, pairs, hp: PreferenceHParams, stat_ptr, coef=None, rewards=None,
+                    ref_logp=None, mask=None, pair_weight=None, flags=0, stream=None):
+    """Preference loss of packed pairs of sequences; ``coef`` receives dloss/dlogp, ``rewards`` beta * s."""
+    check(lib().rlcu_preference_loss(logp_ptr, tokens, ref_logp, mask, offsets_ptr, pairs, pair_weight, C.addressof(hp), coef,
+                                     rewards, stat_ptr, flags, stream))
+
+
+# ---------------------------------------------------------------------------
+# 8-bit activation checkpoints (include/rlcu_act8.h)
+# ---------------------------------------------------------------------------
+
+def act8_blocks(cols) -> int:
+    """Scale bytes of one row."""
+    return lib().rlcu_act8_blocks(cols)
+
+
+def act8_store(x_ptr, dtype, rows, cols, codes_ptr, scales_ptr, x_stride=0, code_stride=0, stream=None):
+    check(lib().rlcu_act8_store(x_ptr, dtype, rows, cols, x_stride, codes_ptr, code_stride, scales_ptr, stream))
+
+
+def act8_load(codes_ptr, scales_ptr, rows, cols, x_ptr, dtype, code_stride=0, x_stride=0, stream=None):
+    check(lib().rlcu_act8_load(codes_ptr, code_stride, scales_ptr, rows, cols, x_ptr, dtype, x_stride, stream))
+
+
+def act8_rmsnorm(codes_ptr, scales_ptr, rows, cols, weight_ptr, weight_dtype, eps, y_ptr, dtype, rstd=None, code_stride=0,
+                 y_stride=0, stream=None):
+    """RMSNorm of a checkpoint's values."""
+    check(lib().rlcu_act8_rmsnorm(codes_ptr, code_stride, scales_ptr, rows, cols, weight_ptr, weight_dtype, eps, y_ptr, dtype,
+                                  y_stride, rstd, stream))
+
+
+def act8_rmsnorm_grad_workspace(rows, cols) -> int:
+    """Bytes of workspace ``act8_rmsnorm_grad`` needs."""
+    return lib().rlcu_act8_rmsnorm_grad_workspace(rows, cols)
+
+
+def act8_rmsnorm_grad(codes_ptr, scales_ptr, rows, cols, weight_ptr, weight_dtype, eps, dy_ptr, dtype, dx_ptr, dweight_ptr,
+                      workspace_ptr, workspace_bytes, dresidual=None, code_stride=0, dy_stride=0, dresidual_stride=0,
+                      dx_stride=0, flags=0, stream=None):
+    """Gradient of that RMSNorm: ``dx`` (plus ``dresidual``) and ``dweight`` (FP32)."""
+    check(lib().rlcu_act8_rmsnorm_grad(codes_ptr, code_stride, scales_ptr, rows, cols, weight_ptr, weight_dtype, eps, dy_ptr,
+                                       dy_stride, dresidual, dresidual_stride, dx_ptr, dx_stride, dtype, dweight_ptr,
+                                       workspace_ptr, workspace_bytes, flags, stream))

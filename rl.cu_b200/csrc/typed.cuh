@@ -1,0 +1,119 @@
+// Element types of the operators that take FP16, bfloat16 or FP32 tensors: 16-byte groups unpacked to FP32
+// and back (one rounding), single elements, and the alignment arithmetic of rows that start anywhere.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "rlcu_adamw.h"
+
+namespace rlcu {
+
+template <uint32_t DT>
+struct Elem {                                   // RLCU_F16 and RLCU_BF16
+    using T = uint16_t;
+    static constexpr int kVec = 8;              // elements of 16 bytes
+    static constexpr bool kBF = DT == RLCU_BF16;
+
+    static __device__ __forceinline__ float up(T x) {
+        return kBF ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
+    }
+    static __device__ __forceinline__ T down(float x) {
+        return kBF ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
+    }
+    static __device__ __forceinline__ void up2(uint32_t w, float& a, float& b) {
+        if (kBF) {
+            a = __uint_as_float(w << 16);
+            b = __uint_as_float(w & 0xFFFF0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+            a = f.x;
+            b = f.y;
+        }
+    }
+    static __device__ __forceinline__ uint32_t down2(float a, float b) {
+        if (kBF) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            return *reinterpret_cast<const uint32_t*>(&h);
+        }
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ void unpack(uint4 x, float (&f)[kVec]) {
+        up2(x.x, f[0], f[1]);
+        up2(x.y, f[2], f[3]);
+        up2(x.z, f[4], f[5]);
+        up2(x.w, f[6], f[7]);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[kVec]) {
+        return make_uint4(down2(f[0], f[1]), down2(f[2], f[3]), down2(f[4], f[5]), down2(f[6], f[7]));
+    }
+    // largest element of 16 bytes (NaN is passed over)
+    static __device__ __forceinline__ float largest(uint4 x) {
+        float a, b;
+        if (kBF) {
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x);
+            const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            up2(*reinterpret_cast<const uint32_t*>(&m), a, b);
+        } else {
+            const __half2* h = reinterpret_cast<const __half2*>(&x);
+            const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            up2(*reinterpret_cast<const uint32_t*>(&m), a, b);
+        }
+        return fmaxf(a, b);
+    }
+};
+
+template <>
+struct Elem<RLCU_F32> {
+    using T = float;
+    static constexpr int kVec = 4;
+    static __device__ __forceinline__ float up(T x) { return x; }
+    static __device__ __forceinline__ T down(float x) { return x; }
+    static __device__ __forceinline__ void unpack(uint4 x, float (&f)[kVec]) {
+        f[0] = __uint_as_float(x.x);
+        f[1] = __uint_as_float(x.y);
+        f[2] = __uint_as_float(x.z);
+        f[3] = __uint_as_float(x.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[kVec]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+    static __device__ __forceinline__ float largest(uint4 x) {
+        return fmaxf(fmaxf(__uint_as_float(x.x), __uint_as_float(x.y)), fmaxf(__uint_as_float(x.z), __uint_as_float(x.w)));
+    }
+};
+
+// A row of n elements cut at 16-byte boundaries: `head` single elements, `groups` groups, then the rest.
+struct RowCut {
+    uint32_t head, groups;
+};
+
+template <typename T>
+__device__ __forceinline__ RowCut cut_row(const T* row, uint32_t n) {
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15u) / (uint32_t)sizeof(T);
+    constexpr uint32_t kVec = 16 / sizeof(T);
+    uint32_t head = off ? kVec - off : 0u;
+    if (head > n) head = n;
+    return {head, (n - head) / kVec};
+}
+
+__host__ inline size_t dtype_bytes(uint32_t dtype) { return dtype == RLCU_F32 ? 4 : 2; }
+__host__ inline bool dtype_known(uint32_t dtype) { return dtype == RLCU_F16 || dtype == RLCU_F32 || dtype == RLCU_BF16; }
+
+// rows of `stride` elements that no address space could hold are refused before any product of the two is formed
+__host__ inline bool too_large(uint64_t rows, uint64_t stride) { return rows && stride > (1ull << 48) / rows; }
+
+// a rows x cols matrix with `stride` elements from row to row, as the bytes from its first to its last element
+struct Span {
+    uintptr_t lo, hi;
+};
+__host__ inline Span span_of(const void* p, uint64_t rows, uint64_t cols, uint64_t stride, size_t esz) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+    return {lo, rows && cols ? lo + ((rows - 1) * stride + cols) * esz : lo};
+}
+__host__ inline bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
+
+}  // namespace rlcu
