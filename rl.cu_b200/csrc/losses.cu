@@ -7,6 +7,8 @@
 //   dz_j = coef * S * t * ([j == y] - 2^x_j / s)
 #include "rlcu_losses.h"
 
+#include <cooperative_groups.h>
+
 #include <cfloat>
 #include <cmath>
 
@@ -18,6 +20,15 @@ namespace {
 
 constexpr int kRowThreads = 512;
 constexpr float kLog2E = 1.4426950408889634f;
+#ifndef WIDE
+#define WIDE 256
+#endif
+#ifndef HELD_CTAS
+#define HELD_CTAS (1024 / THREADS)
+#endif
+#ifndef SUM_DEPTH
+#define SUM_DEPTH 4
+#endif
 constexpr float kLn2 = 0.6931471805599453f;
 // Where the running maximum starts: logits below it (-inf, and masks of a type's lowest value) add nothing,
 // and a row without any other has s = 0.
@@ -55,11 +66,11 @@ struct PolicyTerm {
     bool cut;
 };
 
-// One token of the policy loss.
-__device__ __forceinline__ PolicyTerm policy_term(float logp, const PolicyArgs& p, uint64_t t) {
-    const float a = p.advantage[t], w = p.weight[t];
+// One token of the policy loss: advantage a, weight w, log-probabilities logp, old (p.old_logp given) and ref
+// (a KL term given).
+__device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& p, float logp, float a, float w, float old, float ref) {
     PolicyTerm o;
-    o.ratio = p.old_logp ? expf(logp - p.old_logp[t]) : 1.0f;
+    o.ratio = p.old_logp ? expf(logp - old) : 1.0f;
     const float lo = 1.0f - p.hp.clip_low, hi = 1.0f + p.hp.clip_high;
     const float kept = o.ratio * a;
     float best = kept, slope = kept;
@@ -80,7 +91,7 @@ __device__ __forceinline__ PolicyTerm policy_term(float logp, const PolicyArgs& 
     o.k = 0.0f;
     float dk = 0.0f;
     if (p.hp.kl_coef != 0.0f) {
-        const float d = logp - p.ref_logp[t];
+        const float d = logp - ref;
         if (p.hp.kl_kind == RLCU_KL_K1) {
             o.k = d;
             dk = 1.0f;
@@ -97,22 +108,28 @@ __device__ __forceinline__ PolicyTerm policy_term(float logp, const PolicyArgs& 
     return o;
 }
 
+__device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& p, float logp, uint64_t t) {
+    return policy_term(p, logp, p.advantage[t], p.weight[t], p.old_logp ? p.old_logp[t] : 0.0f,
+                       p.hp.kl_coef != 0.0f ? p.ref_logp[t] : 0.0f);
+}
+
 // ---------------------------------------------------------------------------
 // logits
 // ---------------------------------------------------------------------------
 
-// Sum of 2^(c z - ceil(c max)) with its running maximum.
+// Sum of 2^(c z - e) for an integer e that follows the largest c z: raised when terms pass 2^kSlack, so after a
+// thread's first group hardly ever.  The sum is a float: how far e lies below the largest term costs nothing.
+constexpr float kSlack = 1099511627776.0f;            // 2^40
+
 struct Online {
-    float top = kNoLogit;   // largest logit so far
-    float e;                // ceil(c * top)
+    float e;
     float s = 0.0f;
 
     __device__ __forceinline__ explicit Online(float c) : e(ceilf(kNoLogit * c)) {}
-    __device__ __forceinline__ void raise(float top_new, float c) {
-        if (top_new > top) {
-            const float e_new = ceilf(top_new * c);
+    __device__ __forceinline__ void raise(float largest, float c) {
+        const float e_new = ceilf(largest * c);
+        if (e_new > e) {
             s *= exp2_fast(e - e_new);
-            top = top_new;
             e = e_new;
         }
     }
@@ -121,27 +138,90 @@ struct Online {
         s += exp2_fast(fmaf(z, c, -e));
     }
     template <int N>
-    __device__ __forceinline__ void add(const float (&z)[N], float largest, float c) {
-        raise(largest, c);
-        float a = 0.0f, b = 0.0f;
+    __device__ __forceinline__ float terms(const float (&f)[N], float c) const {
+        const F2 cc(c, c), ee(-e, -e);
+        F2 sum;
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
-            a += exp2_fast(fmaf(z[i], c, -e));
-            b += exp2_fast(fmaf(z[i + 1], c, -e));
+            float x, y;
+            fma2(F2(f[i], f[i + 1]), cc, ee).get(x, y);
+            const F2 term(exp2_fast(x), exp2_fast(y));
+            sum = i ? add2(sum, term) : term;
         }
-        s += a + b;
+        float x, y;
+        sum.get(x, y);
+        return x + y;
     }
-    __device__ __forceinline__ void merge(float top2, float s2, float c) {
-        const float e2 = ceilf(top2 * c);
-        if (top2 > top) {
-            s = s * exp2_fast(e - e2) + s2;
-            top = top2;
-            e = e2;
-        } else {
-            s = s + s2 * exp2_fast(e2 - e);
+    // a group of 16 bytes
+    template <uint32_t DT>
+    __device__ __forceinline__ void add(uint4 v, float c) {
+        using E = Elem<DT>;
+        float f[E::kVec];
+        E::unpack(v, f);
+        float sum = terms(f, c);
+        if (sum > kSlack) {                            // (NaN is not: it goes into the sum)
+            raise(E::largest(v), c);
+            sum = terms(f, c);
+        }
+        s += sum;
+    }
+    __device__ __forceinline__ void merge(float e2, float s2) {
+        const float most = fmaxf(e, e2);
+        s = s * exp2_fast(e - most) + s2 * exp2_fast(e2 - most);
+        e = most;
+    }
+    __device__ __forceinline__ void merge_warp() {
+        float most = e;
+#pragma unroll
+        for (int mask = 16; mask >= 1; mask >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, mask));
+        s *= exp2_fast(e - most);
+        e = most;
+#pragma unroll
+        for (int mask = 16; mask >= 1; mask >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, mask);
+    }
+    // s in [1, 2), or 0, inf or NaN: x_y = c z_y - e is then no larger than its own logarithm
+    __device__ __forceinline__ void settle() {
+        if (s > 0.0f && s < INFINITY) {
+            const int k = (int)((__float_as_uint(s) >> 23) & 0xFFu) - 127;
+            s *= __uint_as_float((uint32_t)(127 - k) << 23);
+            e += (float)k;
         }
     }
 };
+
+// What one thread makes of a row's sum.
+struct RowAnswer {
+    float logp, lse;
+    float e, inv;      // p_j = 2^(c z_j - e) * inv
+};
+
+__device__ __forceinline__ RowAnswer row_answer(Online o, float z_y, float c) {
+    if (o.e == INFINITY) o.s = NAN;           // logits whose product with c is beyond FP32
+    o.settle();
+    const float l2 = log2f(o.s);
+    RowAnswer r;
+    r.logp = o.s == 0.0f ? -INFINITY : (fmaf(z_y, c, -o.e) - l2) * kLn2;      // 0: nothing but -inf in the row
+    r.lse = o.s == 0.0f ? -INFINITY : (o.e + l2) * kLn2;
+    r.e = o.e;
+    r.inv = o.s == 0.0f ? 0.0f : 1.0f / o.s;
+    return r;
+}
+
+// 16 bytes of gradient away from the target: kn 2^(c z - e)
+template <uint32_t DT>
+__device__ __forceinline__ uint4 grad_group(uint4 v, float c, float e, float kn) {
+    using E = Elem<DT>;
+    float f[E::kVec];
+    E::unpack(v, f);
+    const F2 cc(c, c), ee(-e, -e), kk(kn, kn);
+#pragma unroll
+    for (int i = 0; i < E::kVec; i += 2) {
+        float x, y;
+        fma2(F2(f[i], f[i + 1]), cc, ee).get(x, y);
+        mul2(F2(exp2_fast(x), exp2_fast(y)), kk).get(f[i], f[i + 1]);
+    }
+    return E::pack(f);
+}
 
 enum { kModeLogprob = 0, kModeGrad = 1, kModePolicy = 2 };
 
@@ -168,8 +248,8 @@ __global__ void __launch_bounds__(kRowThreads)
 logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* coef_in) {
     using E = Elem<DT>;
     using T = typename E::T;
-    __shared__ float tops[kRowThreads / 32], sums[kRowThreads / 32];
-    __shared__ float row_e, row_scale, row_k;
+    __shared__ float2 warp_part[kRowThreads / 32];
+    __shared__ float4 answer;                         // e, -k / s, k (1 - p_y)
     const float c = a.inv_temperature * kLog2E;
     const float S = a.scaler ? a.scaler->scale : 1.0f;
 
@@ -192,36 +272,24 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
 
         if (MODE != kModeGrad) {
             Online o(c);
-            for (uint32_t i = threadIdx.x; i < cut.groups; i += kRowThreads) {
-                const uint4 v = body[i];
-                float f[E::kVec];
-                E::unpack(v, f);
-                o.add(f, E::largest(v), c);
-            }
+            for (uint32_t i = threadIdx.x; i < cut.groups; i += kRowThreads) o.add<DT>(body[i], c);
             if (threadIdx.x < cut.head) o.add(E::up(x[threadIdx.x]), c);
             for (uint32_t i = tail + threadIdx.x; i < a.vocab; i += kRowThreads) o.add(E::up(x[i]), c);
-#pragma unroll
-            for (int mask = 16; mask >= 1; mask >>= 1)
-                o.merge(__shfl_xor_sync(0xFFFFFFFFu, o.top, mask), __shfl_xor_sync(0xFFFFFFFFu, o.s, mask), c);
-            if ((threadIdx.x & 31) == 0) {
-                tops[threadIdx.x >> 5] = o.top;
-                sums[threadIdx.x >> 5] = o.s;
-            }
+            o.merge_warp();
+            if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = make_float2(o.e, o.s);
             __syncthreads();
-            if (threadIdx.x == 0) {
+            if (threadIdx.x < 32) {
                 Online all(c);
-                for (int w = 0; w < kRowThreads / 32; w++) all.merge(tops[w], sums[w], c);
-                if (all.e == INFINITY) all.s = NAN;      // logits whose product with c is beyond FP32
-                const float l2 = log2f(all.s);
-                // s = 0: nothing but -inf in the row
-                const float logp = all.s == 0.0f ? -INFINITY : (fmaf(E::up(x[y]), c, -all.e) - l2) * kLn2;
-                a.logp[row] = logp;
-                if (a.lse) a.lse[row] = (all.e + l2) * kLn2;
-                if (MODE == kModePolicy) {
-                    row_e = all.e;
-                    row_scale = all.s == 0.0f ? 0.0f : 1.0f / all.s;
-                    row_k = policy_term(logp, p, row).coef * S * a.inv_temperature;
-                    tops[0] = -expm1f(logp);     // 1 - p_y
+                if (threadIdx.x < kRowThreads / 32) all.merge(warp_part[threadIdx.x].x, warp_part[threadIdx.x].y);
+                all.merge_warp();
+                if (threadIdx.x == 0) {
+                    const RowAnswer r = row_answer(all, E::up(x[y]), c);
+                    a.logp[row] = r.logp;
+                    if (a.lse) a.lse[row] = r.lse;
+                    if (MODE == kModePolicy) {
+                        const float k = policy_term(p, r.logp, row).coef * S * a.inv_temperature;
+                        answer = make_float4(r.e, -k * r.inv, -k * expm1f(r.logp), 0.0f);
+                    }
                 }
             }
             __syncthreads();
@@ -229,34 +297,27 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
         if (MODE == kModeLogprob) continue;
 
         // gradient
-        float e, scale, k, rest;
+        float e, kn, ky;
         if (MODE == kModePolicy) {
-            e = row_e;
-            scale = row_scale;
-            k = row_k;
-            rest = tops[0];
+            e = answer.x;
+            kn = answer.y;
+            ky = answer.z;
         } else {
-            const float lse = lse_in[row];
             // 2^(c z - log2e lse) = 2^(c z - e) * 2^(e - log2e lse), e an integer
-            e = lse == -INFINITY ? 0.0f : rintf(lse * kLog2E);
-            scale = lse == -INFINITY ? 0.0f : exp2f(-fmaf(lse, kLog2E, -e));
-            k = coef_in[row] * S * a.inv_temperature;
-            rest = lse == -INFINITY ? 1.0f : -expm1f(fmaf(E::up(x[y]), a.inv_temperature, -lse));
+            const float lse = lse_in[row], k = coef_in[row] * S * a.inv_temperature;
+            const bool empty = lse == -INFINITY;
+            e = empty ? 0.0f : rintf(lse * kLog2E);
+            kn = empty ? 0.0f * k : -k * exp2f(-fmaf(lse, kLog2E, -e));
+            ky = empty ? k : -k * expm1f(fmaf(E::up(x[y]), a.inv_temperature, -lse));
         }
-        const float kn = -k * scale, ky = k * rest;
         if (MODE == kModeGrad) __syncthreads();          // x[y] is read before it is overwritten in place
         T* g = static_cast<T*>(a.grad) + row * a.grad_stride;
         const bool vec = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
         if (vec) {
             uint4* out = reinterpret_cast<uint4*>(g + cut.head);
-            for (uint32_t i = threadIdx.x; i < cut.groups; i += kRowThreads) {
-                float f[E::kVec];
-                E::unpack(body[i], f);
-                const uint32_t at = (uint32_t)y - (cut.head + i * E::kVec);
-#pragma unroll
-                for (int j = 0; j < E::kVec; j++) f[j] = (uint32_t)j == at ? ky : kn * exp2_fast(fmaf(f[j], c, -e));
-                __stcs(out + i, E::pack(f));
-            }
+            for (uint32_t i = threadIdx.x; i < cut.groups; i += kRowThreads) __stcs(out + i, grad_group<DT>(body[i], c, e, kn));
+            if ((uint32_t)y - cut.head < cut.groups * E::kVec && ((uint32_t)y - cut.head) / E::kVec % kRowThreads == threadIdx.x)
+                g[y] = E::down(ky);              // behind this thread's own store of the group
             if (threadIdx.x < cut.head)
                 g[threadIdx.x] = E::down(threadIdx.x == (uint32_t)y ? ky : kn * exp2_fast(fmaf(E::up(x[threadIdx.x]), c, -e)));
             for (uint32_t i = tail + threadIdx.x; i < a.vocab; i += kRowThreads)
@@ -265,8 +326,294 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
             for (uint32_t i = threadIdx.x; i < a.vocab; i += kRowThreads)
                 g[i] = E::down(i == (uint32_t)y ? ky : kn * exp2_fast(fmaf(E::up(x[i]), c, -e)));
         }
-        __syncthreads();                                  // row_* and tops are written again for the next row
+        __syncthreads();                                  // the shared values are written again for the next row
     }
+}
+
+__device__ __forceinline__ void copy_async16(void* smem, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                 :: "r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+constexpr int kMostCluster = 16;
+
+// What decides whether a row takes part.  It is loaded two rows ahead: the two loads' latency, exposed once a row, cost
+// more than the row's arithmetic.
+struct RowFacts {
+    int32_t y;
+    float weight;
+    __device__ __forceinline__ RowFacts(const LogitsArgs& a, const PolicyArgs& p, uint32_t row) {
+        y = row < a.rows ? a.targets[row] : -1;
+        weight = row < a.rows && p.weight ? p.weight[row] : 1.0f;
+    }
+};
+
+// A row's share of one thread of a CTA: every THREADS-th group of the CTA's run, and perhaps one of the single
+// elements at the row's ends.
+template <uint32_t DT, int THREADS>
+struct RowShare {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    uint32_t row;
+    const uint4* in;          // first group
+    uint32_t groups;
+    uint32_t end_at;          // index of the single element, or vocab
+    uint32_t y;
+    bool takes;
+    bool owns_y;              // the target is in one of the groups
+
+    __device__ __forceinline__ RowShare() : row(0), in(nullptr), groups(0), end_at(0), y(0), takes(false), owns_y(false) {}
+    __device__ __forceinline__ RowShare(const LogitsArgs& a, uint32_t row_, RowFacts f, uint32_t rank, uint32_t C) : RowShare() {
+        row = row_;
+        y = (uint32_t)f.y;
+        end_at = a.vocab;
+        takes = y < a.vocab && f.weight != 0.0f;      // (a negative target is above any vocab)
+        if (!takes) return;
+        const T* x = static_cast<const T*>(a.data) + (uint64_t)row * a.row_stride;
+        const RowCut cut = cut_row(x, a.vocab);
+        const uint32_t tid = threadIdx.x, tail = cut.head + cut.groups * E::kVec;
+        const uint32_t share = (cut.groups + C - 1) / C;
+        const uint32_t lo = min(rank * share, cut.groups), n = min(share, cut.groups - lo);
+        groups = n > tid ? (n - tid + THREADS - 1) / THREADS : 0;
+        in = reinterpret_cast<const uint4*>(x + cut.head) + lo + tid;
+        if (rank == 0 && tid < cut.head + (a.vocab - tail)) end_at = tid < cut.head ? tid : tail + (tid - cut.head);
+        const uint32_t group = (y - cut.head) / E::kVec - lo;
+        owns_y = y >= cut.head && y < tail && group < n && group % THREADS == tid;
+    }
+    // a row that takes no part
+    template <int MODE>
+    __device__ __forceinline__ void skip(const LogitsArgs& a, uint32_t rank, uint32_t C) const {
+        if (rank == 0 && threadIdx.x == 0) {
+            a.logp[row] = 0.0f;
+            if (a.lse) a.lse[row] = 0.0f;
+        }
+        if (MODE == kModePolicy) zero_row<DT>(a.grad, (uint64_t)row * a.grad_stride, a.vocab, rank * THREADS + threadIdx.x, C * THREADS);
+    }
+};
+
+// Set when a bounded wait below gave up; read and cleared by rlcu_losses_check.  In host code this name is only a
+// handle for cudaMemcpyFromSymbol.
+static __device__ unsigned int losses_error_word;
+constexpr uint32_t kWaitTries = 1u << 18;
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// Sums of all threads of a cluster, in warp 0 of each of its CTAs.  The CTAs hand each other their sums with st.async,
+// whose arrival the receiver's mbarrier counts in bytes: unlike a cluster barrier with release semantics this does not
+// wait for the gradient stores that are still on their way (which took longer than the row's arithmetic: 667 us
+// instead of ~ for 4096 x 151936 bf16).
+template <int WARPS>
+struct ClusterSum {
+    float2 warp_part[2][WARPS];            // by row parity: the warps may be a row ahead of the one that reads
+    float2 part[2][kMostCluster];          // (e, s) of each CTA
+    unsigned long long bar[2];
+
+    __device__ __forceinline__ void init(uint32_t C) {
+        if (C == 1) return;
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < 2; i++)
+                asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(smem_at(&bar[i])) : "memory");
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        cluster_barrier();
+    }
+    // a CTA leaves when no other one of its cluster can still write to it
+    __device__ __forceinline__ void finish(uint32_t C) {
+        if (C > 1) cluster_barrier();
+    }
+    static __device__ __forceinline__ void cluster_barrier() {
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    // every warp, row n (counted from 0): what it has of the sum
+    __device__ __forceinline__ void give(Online o, uint32_t n) {
+        o.merge_warp();
+        if ((threadIdx.x & 31) == 0) warp_part[n & 1][threadIdx.x >> 5] = make_float2(o.e, o.s);
+    }
+    // one warp, behind a barrier with all that give: the sum over the cluster
+    __device__ __forceinline__ Online take(float c, uint32_t n, uint32_t rank, uint32_t C) {
+        const uint32_t lane = threadIdx.x & 31, parity = n & 1, phase = (n >> 1) & 1;
+        Online o(c);
+        if (lane < WARPS) o.merge(warp_part[parity][lane].x, warp_part[parity][lane].y);
+        o.merge_warp();                                      // every lane has the sum: lane r hands it to CTA r
+        if (C == 1) return o;
+        const uint32_t here = smem_at(&bar[parity]);
+        if (lane == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(here), "r"(C * 8u) : "memory");
+        if (lane < C) {
+            uint32_t to, to_bar;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_at(&part[parity][rank])), "r"(lane));
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to_bar) : "r"(here), "r"(lane));
+            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];"
+                         :: "r"(to), "f"(o.e), "f"(o.s), "r"(to_bar) : "memory");
+        }
+        uint32_t done = 0;
+        for (uint32_t i = 0; i < kWaitTries && !done; i++)
+            asm volatile(
+                "{\n"
+                ".reg .pred p;\n"
+                "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+                "selp.u32 %0, 1, 0, p;\n"
+                "}\n"
+                : "=r"(done) : "r"(here), "r"(phase) : "memory");
+        o = Online(c);
+        if (!done) {                                         // gave up: the row's results are NaN
+            if (lane == 0) atomicExch(&losses_error_word, 1u);
+            o.s = NAN;
+        } else if (lane < C) {
+            o.merge(part[parity][lane].x, part[parity][lane].y);
+        }
+        __syncwarp();
+        o.merge_warp();
+        return o;
+    }
+};
+
+// The policy loss of most calls.  A row belongs to a cluster of C CTAs, each of which has a run of its 16-byte groups
+// and keeps it in registers between the sum and the gradient: the logits are read once, the gradient is written once.
+// Several clusters share an SM, so that one row's loads and stores run under another's arithmetic.
+template <uint32_t DT, int THREADS, int NV>
+__global__ void __launch_bounds__(THREADS, HELD_CTAS)
+logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    __shared__ ClusterSum<THREADS / 32> sums;
+    __shared__ float inputs[8];
+    __shared__ float4 answer;                         // e, -k / s, k (1 - p_y)
+    const uint32_t C = cooperative_groups::this_cluster().num_blocks(), rank = cooperative_groups::this_cluster().block_rank();
+    const int tid = threadIdx.x;
+    const float c = a.inv_temperature * kLog2E;
+    const uint32_t step = gridDim.x / C;
+    uint32_t n = 0;
+    bool ready = false;
+    for (uint32_t row = blockIdx.x / C; row < a.rows; row += step) {
+        const RowShare<DT, THREADS> now(a, row, RowFacts(a, p, row), rank, C);
+        if (!now.takes) {
+            now.template skip<kModePolicy>(a, rank, C);
+            continue;
+        }
+        const T* x = static_cast<const T*>(a.data) + (uint64_t)row * a.row_stride;
+        uint4 v[NV];
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            if (j < (int)now.groups) v[j] = __ldcs(now.in + j * THREADS);
+        float end = 0.0f, input = 0.0f;
+        if (now.end_at < a.vocab) end = E::up(x[now.end_at]);
+        if (tid == 32) input = E::up(x[now.y]);
+        if (tid == 33) input = p.advantage[row];
+        if (tid == 34) input = p.weight[row];
+        if (tid == 35 && p.old_logp) input = p.old_logp[row];
+        if (tid == 36 && p.hp.kl_coef != 0.0f) input = p.ref_logp[row];
+        if (!ready) sums.init(C);                     // under the loads
+        ready = true;
+        Online o(c);
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            if (j < (int)now.groups) o.add<DT>(v[j], c);
+        if (now.end_at < a.vocab) o.add(end, c);
+        if (tid >= 32 && tid < 37) inputs[tid - 32] = input;
+        sums.give(o, n);
+        __syncthreads();
+        if (tid < 32) {
+            o = sums.take(c, n, rank, C);
+            if (tid == 0) {
+                const RowAnswer r = row_answer(o, inputs[0], c);
+                if (rank == 0) a.logp[row] = r.logp;
+                const float S = a.scaler ? a.scaler->scale : 1.0f;
+                const float k = policy_term(p, r.logp, inputs[1], inputs[2], inputs[3], inputs[4]).coef * S * a.inv_temperature;
+                answer = make_float4(r.e, -k * r.inv, -k * expm1f(r.logp), 0.0f);
+            }
+        }
+        __syncthreads();
+        const float e = answer.x, kn = answer.y, ky = answer.z;
+        T* g = static_cast<T*>(a.grad) + (uint64_t)row * a.grad_stride;
+        // the gradient's groups lie where the logits' do
+        uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(now.in) + reinterpret_cast<uintptr_t>(g) - reinterpret_cast<uintptr_t>(x));
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            // the packed group is what stays in registers, not what the sum unpacked from it
+            asm volatile("" : "+r"(v[j].x), "+r"(v[j].y), "+r"(v[j].z), "+r"(v[j].w));
+            if (j < (int)now.groups) __stcs(out + j * THREADS, grad_group<DT>(v[j], c, e, kn));
+        }
+        if (now.end_at < a.vocab) g[now.end_at] = E::down(now.end_at == now.y ? ky : kn * exp2_fast(fmaf(end, c, -e)));
+        if (now.owns_y) g[now.y] = E::down(ky);       // behind this thread's own store of the group
+        n++;
+    }
+    if (ready) sums.finish(C);
+}
+
+// Log-probabilities alone: a cluster (one CTA, unless rows are few) sums row after row, kDepth groups per thread on their
+// way in a ring of slots.
+constexpr int kDepth = SUM_DEPTH;
+
+template <uint32_t DT, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    extern __shared__ uint4 slots[];                  // [kDepth][THREADS]
+    __shared__ ClusterSum<THREADS / 32> sums;
+    __shared__ float z_y[2];                          // by row parity, as the warps' sums
+    const uint32_t C = cooperative_groups::this_cluster().num_blocks(), rank = cooperative_groups::this_cluster().block_rank();
+    const int tid = threadIdx.x;
+    const float c = a.inv_temperature * kLog2E;
+    uint4* mine = slots + tid;
+    const uint32_t step = gridDim.x / C;
+    uint32_t n = 0;
+    sums.init(C);
+
+    auto first = [&](const RowShare<DT, THREADS>& r) {
+#pragma unroll
+        for (int d = 0; d < kDepth; d++) {
+            if ((uint32_t)d < r.groups) copy_async16(mine + d * THREADS, r.in + d * THREADS);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    };
+    RowShare<DT, THREADS> now(a, blockIdx.x / C, RowFacts(a, p, blockIdx.x / C), rank, C);
+    RowFacts ahead(a, p, now.row + step);
+    first(now);
+    while (now.row < a.rows) {
+        const RowShare<DT, THREADS> next(a, now.row + step, ahead, rank, C);
+        ahead = RowFacts(a, p, now.row + 2 * step);
+        const T* x = static_cast<const T*>(a.data) + (uint64_t)now.row * a.row_stride;
+        float end = 0.0f, input = 0.0f;
+        if (now.end_at < a.vocab) end = E::up(x[now.end_at]);
+        if (tid == 32 && now.takes) input = E::up(x[now.y]);
+        Online o(c);
+        const uint4* in = now.in + kDepth * THREADS;
+        for (uint32_t j0 = 0; j0 < now.groups; j0 += kDepth) {
+#pragma unroll
+            for (int d = 0; d < kDepth; d++) {
+                if (j0 + d < now.groups) {
+                    asm volatile("cp.async.wait_group %0;" :: "n"(kDepth - 1) : "memory");
+                    o.add<DT>(mine[d * THREADS], c);
+                    if (j0 + d + kDepth < now.groups) copy_async16(mine + d * THREADS, in + d * THREADS);
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                }
+            }
+            in += kDepth * THREADS;
+        }
+        first(next);
+        if (now.takes) {
+            if (now.end_at < a.vocab) o.add(end, c);
+            if (tid == 32) z_y[n & 1] = input;
+            sums.give(o, n);
+            __syncthreads();
+            if (tid < 32) {
+                o = sums.take(c, n, rank, C);
+                if (tid == 0 && rank == 0) {
+                    const RowAnswer r = row_answer(o, z_y[n & 1], c);
+                    a.logp[now.row] = r.logp;
+                    if (a.lse) a.lse[now.row] = r.lse;
+                }
+            }
+            n++;
+        } else {
+            now.template skip<kModeLogprob>(a, rank, C);
+        }
+        now = next;
+    }
+    sums.finish(C);
 }
 
 // ---------------------------------------------------------------------------
@@ -299,7 +646,7 @@ policy_kernel(const float* logp, uint64_t tokens, const int32_t* targets, uint32
         const bool takes = w != 0.0f && (!targets || (targets[t] >= 0 && (uint32_t)targets[t] < vocab));
         float co = 0.0f;
         if (takes) {
-            const PolicyTerm o = policy_term(logp[t], p, t);
+            const PolicyTerm o = policy_term(p, logp[t], t);
             sum_l += (double)w * o.l;
             sum_k += (double)w * o.k;
             sum_w += w;
@@ -505,6 +852,78 @@ int launch_rows(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, const 
     return RLCU_OK;
 }
 
+template <typename Kernel>
+int launch_clusters(Kernel kernel, const LogitsArgs& a, const PolicyArgs& p, int cluster, int threads, int smem, cudaStream_t s) {
+    RLCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (cluster > 8) RLCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int most = 0;
+    RLCU_CUDA(cudaOccupancyMaxActiveClusters(&most, kernel, &cfg));
+    if (most < 1) return set_error(RLCU_ERR_CUDA, "kernel does not fit on an SM");
+#ifdef EACH
+    if (smem == 0) most = 1 << 24;
+#endif
+    cfg.gridDim = dim3((unsigned)((a.rows < (uint64_t)most ? a.rows : (uint64_t)most) * cluster));
+    RLCU_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, p));
+    return RLCU_OK;
+}
+
+constexpr int kWide = WIDE, kNarrow = 128, kMostHeld = 10;
+
+template <uint32_t DT, int THREADS>
+int launch_policy_rows(const LogitsArgs& a, const PolicyArgs& p, int cluster, uint32_t held, cudaStream_t s) {
+#define RLCU_HELD(NV) \
+    if (held <= NV) return launch_clusters(logits_policy_kernel<DT, THREADS, NV>, a, p, cluster, THREADS, 0, s)
+    RLCU_HELD(2);
+    RLCU_HELD(4);
+    RLCU_HELD(6);
+    RLCU_HELD(8);
+    RLCU_HELD(10);
+#undef RLCU_HELD
+    return set_error(RLCU_ERR_UNSUPPORTED, "row too long");
+}
+
+template <uint32_t DT, int MODE>
+int launch_logits_dt(const LogitsArgs& a, const PolicyArgs& p, int sms, uint64_t groups, cudaStream_t s) {
+    const int threads = MODE == kModePolicy ? (groups > kNarrow * kMostHeld ? kWide : kNarrow) : (groups > 1024 ? 256 : kNarrow);
+    int cluster = 1;
+    if (MODE == kModePolicy)
+        while (cluster < kMostCluster && groups > (uint64_t)cluster * threads * kMostHeld) cluster *= 2;
+    while (cluster < 8 && a.rows * cluster < (uint64_t)sms && groups > (uint64_t)cluster * threads) cluster *= 2;
+    if (MODE == kModePolicy) {
+        const uint32_t held = (uint32_t)(((groups + cluster - 1) / cluster + threads - 1) / threads);
+        return threads == kWide ? launch_policy_rows<DT, kWide>(a, p, cluster, held, s) : launch_policy_rows<DT, kNarrow>(a, p, cluster, held, s);
+    }
+    return threads == 256 ? launch_clusters(logits_sum_kernel<DT, 256>, a, p, cluster, 256, kDepth * 256 * 16, s)
+                          : launch_clusters(logits_sum_kernel<DT, kNarrow>, a, p, cluster, kNarrow, kDepth * kNarrow * 16, s);
+}
+
+template <int MODE>
+int launch_logits(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, cudaStream_t s) {
+    int sms = 0;
+    if (const int rc = sm_count(&sms)) return rc;
+    const size_t esz = dtype_bytes(dtype);
+    const uint64_t groups = a.vocab / (16 / esz);
+    // every row of the gradient starts at the same place of a 16-byte group as its logits do
+    const bool alike = MODE != kModePolicy || (((reinterpret_cast<uintptr_t>(a.grad) ^ reinterpret_cast<uintptr_t>(a.data)) & 15) == 0 &&
+                                               (a.grad_stride - a.row_stride) * esz % 16 == 0);
+    const bool fits = MODE != kModePolicy || groups <= (uint64_t)kMostCluster * kWide * kMostHeld;
+    if (!alike || !fits || groups < 64) return launch_rows<MODE>(a, p, dtype, nullptr, nullptr, s);
+    if (dtype == RLCU_F16) return launch_logits_dt<RLCU_F16, MODE>(a, p, sms, groups, s);
+    if (dtype == RLCU_BF16) return launch_logits_dt<RLCU_BF16, MODE>(a, p, sms, groups, s);
+    return launch_logits_dt<RLCU_F32, MODE>(a, p, sms, groups, s);
+}
+
 int launch_policy(const float* logp, uint64_t tokens, const int32_t* targets, uint32_t vocab, const PolicyArgs& p,
                   float* coef, rlcu_policy_stat* stat, uint32_t flags, cudaStream_t s) {
     policy_kernel<<<1, kVectorThreads, 0, s>>>(logp, tokens, targets, vocab, p, coef, stat, flags);
@@ -523,7 +942,7 @@ extern "C" int rlcu_token_logprob(const void* logits, uint32_t dtype, uint64_t r
     if (rows && !logp) return set_error(RLCU_ERR_INVALID, "null logp");
     if (!rows) return RLCU_OK;
     LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, logp, lse, nullptr, 0, nullptr};
-    return launch_rows<kModeLogprob>(a, PolicyArgs{}, dtype, nullptr, nullptr, (cudaStream_t)stream);
+    return launch_logits<kModeLogprob>(a, PolicyArgs{}, dtype, (cudaStream_t)stream);
 }
 
 extern "C" int rlcu_token_logprob_grad(const void* logits, uint32_t dtype, uint64_t rows, uint64_t vocab,
@@ -560,8 +979,8 @@ extern "C" int rlcu_policy_loss(const void* logits, uint32_t dtype, uint64_t row
     LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, logp, nullptr, grad, grad_stride, scaler};
     PolicyArgs p = {old_logp, ref_logp, advantage, weight, *hp};
     if (rows) {
-        const int rc = grad ? launch_rows<kModePolicy>(a, p, dtype, nullptr, nullptr, (cudaStream_t)stream)
-                            : launch_rows<kModeLogprob>(a, p, dtype, nullptr, nullptr, (cudaStream_t)stream);
+        const int rc = grad ? launch_logits<kModePolicy>(a, p, dtype, (cudaStream_t)stream)
+                            : launch_logits<kModeLogprob>(a, p, dtype, (cudaStream_t)stream);
         if (rc) return rc;
     }
     return launch_policy(logp, rows, targets, (uint32_t)vocab, p, nullptr, stat, flags, (cudaStream_t)stream);
