@@ -29,6 +29,9 @@ constexpr float kLog2E = 1.4426950408889634f;
 #ifndef SUM_DEPTH
 #define SUM_DEPTH 4
 #endif
+#ifndef SUM_CTAS
+#define SUM_CTAS 1
+#endif
 constexpr float kLn2 = 0.6931471805599453f;
 // Where the running maximum starts: logits below it (-inf, and masks of a type's lowest value) add nothing,
 // and a row without any other has s = 0.
@@ -223,6 +226,7 @@ __device__ __forceinline__ uint4 grad_group(uint4 v, float c, float e, float kn)
     return E::pack(f);
 }
 
+constexpr uint32_t kNoTarget = 0xFFFFFFFFu;
 enum { kModeLogprob = 0, kModeGrad = 1, kModePolicy = 2 };
 
 __device__ __forceinline__ bool row_takes_part(const LogitsArgs& a, const PolicyArgs& p, uint64_t row, int32_t y) {
@@ -338,39 +342,28 @@ __device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_
 
 constexpr int kMostCluster = 16;
 
-// What decides whether a row takes part.  It is loaded two rows ahead: the two loads' latency, exposed once a row, cost
-// more than the row's arithmetic.
-struct RowFacts {
-    int32_t y;
-    float weight;
-    __device__ __forceinline__ RowFacts(const LogitsArgs& a, const PolicyArgs& p, uint32_t row) {
-        y = row < a.rows ? a.targets[row] : -1;
-        weight = row < a.rows && p.weight ? p.weight[row] : 1.0f;
-    }
-};
-
 // A row's share of one thread of a CTA: every THREADS-th group of the CTA's run, and perhaps one of the single
 // elements at the row's ends.
 template <uint32_t DT, int THREADS>
 struct RowShare {
     using E = Elem<DT>;
     using T = typename E::T;
-    uint32_t row;
+    const T* x;
     const uint4* in;          // first group
+    uint32_t y;
     uint32_t groups;
     uint32_t end_at;          // index of the single element, or vocab
-    uint32_t y;
-    bool takes;
     bool owns_y;              // the target is in one of the groups
 
-    __device__ __forceinline__ RowShare() : row(0), in(nullptr), groups(0), end_at(0), y(0), takes(false), owns_y(false) {}
-    __device__ __forceinline__ RowShare(const LogitsArgs& a, uint32_t row_, RowFacts f, uint32_t rank, uint32_t C) : RowShare() {
-        row = row_;
-        y = (uint32_t)f.y;
+    // y_: the target, below vocab where the row takes part; a row that does not has nothing
+    __device__ __forceinline__ RowShare(const LogitsArgs& a, uint32_t row, uint32_t y_, uint32_t rank, uint32_t C) {
+        y = y_;
+        x = static_cast<const T*>(a.data) + (uint64_t)row * a.row_stride;
+        in = nullptr;
+        groups = 0;
         end_at = a.vocab;
-        takes = y < a.vocab && f.weight != 0.0f;      // (a negative target is above any vocab)
-        if (!takes) return;
-        const T* x = static_cast<const T*>(a.data) + (uint64_t)row * a.row_stride;
+        owns_y = false;
+        if (y >= a.vocab) return;
         const RowCut cut = cut_row(x, a.vocab);
         const uint32_t tid = threadIdx.x, tail = cut.head + cut.groups * E::kVec;
         const uint32_t share = (cut.groups + C - 1) / C;
@@ -381,15 +374,6 @@ struct RowShare {
         const uint32_t group = (y - cut.head) / E::kVec - lo;
         owns_y = y >= cut.head && y < tail && group < n && group % THREADS == tid;
     }
-    // a row that takes no part
-    template <int MODE>
-    __device__ __forceinline__ void skip(const LogitsArgs& a, uint32_t rank, uint32_t C) const {
-        if (rank == 0 && threadIdx.x == 0) {
-            a.logp[row] = 0.0f;
-            if (a.lse) a.lse[row] = 0.0f;
-        }
-        if (MODE == kModePolicy) zero_row<DT>(a.grad, (uint64_t)row * a.grad_stride, a.vocab, rank * THREADS + threadIdx.x, C * THREADS);
-    }
 };
 
 // Set when a bounded wait below gave up; read and cleared by rlcu_losses_check.  In host code this name is only a
@@ -399,14 +383,28 @@ constexpr uint32_t kWaitTries = 1u << 18;
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// bounded wait for a phase of an mbarrier of this CTA
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t phase) {
+    uint32_t done = 0;
+    for (uint32_t i = 0; i < kWaitTries && !done; i++)
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(done) : "r"(bar), "r"(phase) : "memory");
+    return done;
+}
+
 // Sums of all threads of a cluster, in warp 0 of each of its CTAs.  The CTAs hand each other their sums with st.async,
 // whose arrival the receiver's mbarrier counts in bytes: unlike a cluster barrier with release semantics this does not
 // wait for the gradient stores that are still on their way (which took longer than the row's arithmetic: 667 us
 // instead of ~ for 4096 x 151936 bf16).
 template <int WARPS>
 struct ClusterSum {
-    float2 warp_part[2][WARPS];            // by row parity: the warps may be a row ahead of the one that reads
-    float2 part[2][kMostCluster];          // (e, s) of each CTA
+    float2 part[2][kMostCluster * WARPS];  // (e, s) of each warp of the cluster, by row parity: a CTA may be a row ahead
+    uint2 next[2];                         // what warp 0 of the first CTA passes on
     unsigned long long bar[2];
 
     __device__ __forceinline__ void init(uint32_t C) {
@@ -425,47 +423,88 @@ struct ClusterSum {
     static __device__ __forceinline__ void cluster_barrier() {
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
-    // every warp, row n (counted from 0): what it has of the sum
-    __device__ __forceinline__ void give(Online o, uint32_t n) {
+    // every warp, row n (counted from 0): hands what it has of the sum to warp 0 of every CTA
+    __device__ __forceinline__ void give(Online o, uint2 pass_on, uint32_t n, uint32_t rank, uint32_t C) {
+        const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, parity = n & 1;
         o.merge_warp();
-        if ((threadIdx.x & 31) == 0) warp_part[n & 1][threadIdx.x >> 5] = make_float2(o.e, o.s);
-    }
-    // one warp, behind a barrier with all that give: the sum over the cluster
-    __device__ __forceinline__ Online take(float c, uint32_t n, uint32_t rank, uint32_t C) {
-        const uint32_t lane = threadIdx.x & 31, parity = n & 1, phase = (n >> 1) & 1;
-        Online o(c);
-        if (lane < WARPS) o.merge(warp_part[parity][lane].x, warp_part[parity][lane].y);
-        o.merge_warp();                                      // every lane has the sum: lane r hands it to CTA r
-        if (C == 1) return o;
+        if (C == 1) {
+            if (lane == 0) part[parity][warp] = make_float2(o.e, o.s);
+            if (threadIdx.x == 0) next[parity] = pass_on;
+            return;
+        }
         const uint32_t here = smem_at(&bar[parity]);
-        if (lane == 0)
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(here), "r"(C * 8u) : "memory");
+        if (threadIdx.x == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(here), "r"(C * WARPS * 8u + 8u) : "memory");
         if (lane < C) {
             uint32_t to, to_bar;
-            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_at(&part[parity][rank])), "r"(lane));
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_at(&part[parity][rank * WARPS + warp])), "r"(lane));
             asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to_bar) : "r"(here), "r"(lane));
             asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];"
                          :: "r"(to), "f"(o.e), "f"(o.s), "r"(to_bar) : "memory");
+            if (rank == 0 && warp == 0) {
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_at(&next[parity])), "r"(lane));
+                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.u32 [%0], {%1, %2}, [%3];"
+                             :: "r"(to), "r"(pass_on.x), "r"(pass_on.y), "r"(to_bar) : "memory");
+            }
         }
-        uint32_t done = 0;
-        for (uint32_t i = 0; i < kWaitTries && !done; i++)
-            asm volatile(
-                "{\n"
-                ".reg .pred p;\n"
-                "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-                "selp.u32 %0, 1, 0, p;\n"
-                "}\n"
-                : "=r"(done) : "r"(here), "r"(phase) : "memory");
-        o = Online(c);
+    }
+    // warp 0 (C = 1: behind a barrier with all that give): the sum over the cluster
+    __device__ __forceinline__ Online take(float c, uint32_t n, uint32_t C) {
+        const uint32_t lane = threadIdx.x & 31, parity = n & 1, phase = (n >> 1) & 1;
+        const bool done = C == 1 || wait_phase(smem_at(&bar[parity]), phase);
+        Online o(c);
         if (!done) {                                         // gave up: the row's results are NaN
-            if (lane == 0) atomicExch(&losses_error_word, 1u);
+            if (lane == 0) {
+                atomicExch(&losses_error_word, 1u);
+                next[parity] = make_uint2(0xFFFFFFFFu, 0u);
+            }
             o.s = NAN;
-        } else if (lane < C) {
-            o.merge(part[parity][lane].x, part[parity][lane].y);
+        } else {
+            for (uint32_t i = lane; i < C * WARPS; i += 32) o.merge(part[parity][i].x, part[parity][i].y);
         }
         __syncwarp();
         o.merge_warp();
         return o;
+    }
+};
+
+// The rows of a grid with one cluster per row, for clusters that stay: instead of leaving, a cluster takes over the
+// next one that has not been launched.  So rows are worked on in order, by whoever is free, and the addresses in use
+// stay close together: DRAM moves a copy of this shape in 338 us that way and in 394 us when each cluster takes every
+// n-th row and they drift apart.  One thread of the cluster asks.
+struct RowFeed {
+    ulonglong2 response;
+    unsigned long long bar;
+
+    __device__ __forceinline__ void init() {
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(smem_at(&bar)) : "memory");
+    }
+    __device__ __forceinline__ void ask() {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the last response has been read
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], 16;" :: "r"(smem_at(&bar)) : "memory");
+        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                     :: "r"(smem_at(&response)), "r"(smem_at(&bar)) : "memory");
+    }
+    // first CTA of the cluster taken over by request n, or -1: none was left
+    __device__ __forceinline__ int answer(uint32_t n) {
+        if (!wait_phase(smem_at(&bar), n & 1)) {
+            atomicExch(&losses_error_word, 1u);
+            return -1;
+        }
+        unsigned long long lo, hi;
+        int first;
+        asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(smem_at(&response)) : "memory");
+        asm volatile(
+            "{\n"
+            ".reg .b128 h;\n"
+            ".reg .pred p;\n"
+            "mov.b128 h, {%1, %2};\n"
+            "mov.b32 %0, -1;\n"
+            "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+            "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n"
+            "}\n"
+            : "=r"(first) : "l"(lo), "l"(hi) : "memory");
+        return first;
     }
 };
 
@@ -478,140 +517,150 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
     using E = Elem<DT>;
     using T = typename E::T;
     __shared__ ClusterSum<THREADS / 32> sums;
+    __shared__ RowFeed feed;
     __shared__ float inputs[8];
     __shared__ float4 answer;                         // e, -k / s, k (1 - p_y)
     const uint32_t C = cooperative_groups::this_cluster().num_blocks(), rank = cooperative_groups::this_cluster().block_rank();
     const int tid = threadIdx.x;
+    const bool asks = rank == 0 && tid == 0;
     const float c = a.inv_temperature * kLog2E;
-    const uint32_t step = gridDim.x / C;
-    uint32_t n = 0;
-    bool ready = false;
-    for (uint32_t row = blockIdx.x / C; row < a.rows; row += step) {
-        const RowShare<DT, THREADS> now(a, row, RowFacts(a, p, row), rank, C);
-        if (!now.takes) {
-            now.template skip<kModePolicy>(a, rank, C);
-            continue;
-        }
-        const T* x = static_cast<const T*>(a.data) + (uint64_t)row * a.row_stride;
+    if (asks) feed.init();
+    sums.init(C);
+    uint32_t row = blockIdx.x / C;
+    uint32_t y = row_takes_part(a, p, row, a.targets[row]) ? (uint32_t)a.targets[row] : kNoTarget;
+    for (uint32_t n = 0;; n++) {
+        if (asks) feed.ask();
+        const RowShare<DT, THREADS> now(a, row, y, rank, C);
+        T* g = static_cast<T*>(a.grad) + (uint64_t)row * a.grad_stride;
         uint4 v[NV];
 #pragma unroll
         for (int j = 0; j < NV; j++)
             if (j < (int)now.groups) v[j] = __ldcs(now.in + j * THREADS);
         float end = 0.0f, input = 0.0f;
-        if (now.end_at < a.vocab) end = E::up(x[now.end_at]);
-        if (tid == 32) input = E::up(x[now.y]);
-        if (tid == 33) input = p.advantage[row];
-        if (tid == 34) input = p.weight[row];
-        if (tid == 35 && p.old_logp) input = p.old_logp[row];
-        if (tid == 36 && p.hp.kl_coef != 0.0f) input = p.ref_logp[row];
-        if (!ready) sums.init(C);                     // under the loads
-        ready = true;
+        if (now.end_at < a.vocab) end = E::up(now.x[now.end_at]);
+        if (y < a.vocab) {
+            if (tid == 32) input = E::up(now.x[y]);
+            if (tid == 33) input = p.advantage[row];
+            if (tid == 34) input = p.weight[row];
+            if (tid == 35 && p.old_logp) input = p.old_logp[row];
+            if (tid == 36 && p.hp.kl_coef != 0.0f) input = p.ref_logp[row];
+        } else {
+            zero_row<DT>(a.grad, (uint64_t)row * a.grad_stride, a.vocab, rank * THREADS + tid, C * THREADS);
+        }
         Online o(c);
+        uint2 next = make_uint2(0xFFFFFFFFu, kNoTarget);
+        float next_weight = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NV; j++)
+        for (int j = 0; j < NV; j++) {
             if (j < (int)now.groups) o.add<DT>(v[j], c);
+            if (j == 0 && asks) {
+                const int first = feed.answer(n);
+                if (first >= 0) {
+                    next.x = (uint32_t)first / C;
+                    next.y = (uint32_t)a.targets[next.x];
+                    next_weight = p.weight[next.x];
+                }
+            }
+        }
+        if (asks && next_weight == 0.0f) next.y = kNoTarget;
         if (now.end_at < a.vocab) o.add(end, c);
         if (tid >= 32 && tid < 37) inputs[tid - 32] = input;
-        sums.give(o, n);
+        if (tid < 32) {
+            next.x = __shfl_sync(0xFFFFFFFFu, next.x, 0);
+            next.y = __shfl_sync(0xFFFFFFFFu, next.y, 0);
+        }
+        sums.give(o, next, n, rank, C);
         __syncthreads();
         if (tid < 32) {
-            o = sums.take(c, n, rank, C);
-            if (tid == 0) {
+            o = sums.take(c, n, C);
+            if (tid == 0 && y < a.vocab) {
                 const RowAnswer r = row_answer(o, inputs[0], c);
                 if (rank == 0) a.logp[row] = r.logp;
                 const float S = a.scaler ? a.scaler->scale : 1.0f;
                 const float k = policy_term(p, r.logp, inputs[1], inputs[2], inputs[3], inputs[4]).coef * S * a.inv_temperature;
                 answer = make_float4(r.e, -k * r.inv, -k * expm1f(r.logp), 0.0f);
+            } else if (asks) {
+                a.logp[row] = 0.0f;
             }
         }
         __syncthreads();
         const float e = answer.x, kn = answer.y, ky = answer.z;
-        T* g = static_cast<T*>(a.grad) + (uint64_t)row * a.grad_stride;
         // the gradient's groups lie where the logits' do
-        uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(now.in) + reinterpret_cast<uintptr_t>(g) - reinterpret_cast<uintptr_t>(x));
+        uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(now.in) + reinterpret_cast<uintptr_t>(g) -
+                                              reinterpret_cast<uintptr_t>(now.x));
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             // the packed group is what stays in registers, not what the sum unpacked from it
             asm volatile("" : "+r"(v[j].x), "+r"(v[j].y), "+r"(v[j].z), "+r"(v[j].w));
             if (j < (int)now.groups) __stcs(out + j * THREADS, grad_group<DT>(v[j], c, e, kn));
         }
-        if (now.end_at < a.vocab) g[now.end_at] = E::down(now.end_at == now.y ? ky : kn * exp2_fast(fmaf(end, c, -e)));
-        if (now.owns_y) g[now.y] = E::down(ky);       // behind this thread's own store of the group
-        n++;
+        if (now.end_at < a.vocab) g[now.end_at] = E::down(now.end_at == y ? ky : kn * exp2_fast(fmaf(end, c, -e)));
+        if (now.owns_y) g[y] = E::down(ky);           // behind this thread's own store of the group
+        row = sums.next[n & 1].x;
+        y = sums.next[n & 1].y;
+        if (row >= a.rows) break;
     }
-    if (ready) sums.finish(C);
+    sums.finish(C);
 }
 
-// Log-probabilities alone: a cluster (one CTA, unless rows are few) sums row after row, kDepth groups per thread on their
-// way in a ring of slots.
+// Log-probabilities alone: a cluster (one CTA, unless rows are few) per row, kDepth groups per thread on their way in a
+// ring of slots.
 constexpr int kDepth = SUM_DEPTH;
 
 template <uint32_t DT, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, SUM_CTAS)
 logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
     using E = Elem<DT>;
-    using T = typename E::T;
     extern __shared__ uint4 slots[];                  // [kDepth][THREADS]
     __shared__ ClusterSum<THREADS / 32> sums;
-    __shared__ float z_y[2];                          // by row parity, as the warps' sums
+    __shared__ float z_y;
     const uint32_t C = cooperative_groups::this_cluster().num_blocks(), rank = cooperative_groups::this_cluster().block_rank();
     const int tid = threadIdx.x;
     const float c = a.inv_temperature * kLog2E;
     uint4* mine = slots + tid;
-    const uint32_t step = gridDim.x / C;
-    uint32_t n = 0;
+    const uint32_t row = blockIdx.x / C;
+    const int32_t y = a.targets[row];
+    if (!row_takes_part(a, p, row, y)) {              // (the whole cluster)
+        if (rank == 0 && tid == 0) {
+            a.logp[row] = 0.0f;
+            if (a.lse) a.lse[row] = 0.0f;
+        }
+        return;
+    }
+    const RowShare<DT, THREADS> now(a, row, (uint32_t)y, rank, C);
+#pragma unroll
+    for (int d = 0; d < kDepth; d++) {
+        if ((uint32_t)d < now.groups) copy_async16(mine + d * THREADS, now.in + d * THREADS);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    float end = 0.0f;
+    if (now.end_at < a.vocab) end = E::up(now.x[now.end_at]);
+    if (tid == 32) z_y = E::up(now.x[y]);
     sums.init(C);
-
-    auto first = [&](const RowShare<DT, THREADS>& r) {
+    Online o(c);
+    const uint4* in = now.in + kDepth * THREADS;
+    for (uint32_t j0 = 0; j0 < now.groups; j0 += kDepth) {
 #pragma unroll
         for (int d = 0; d < kDepth; d++) {
-            if ((uint32_t)d < r.groups) copy_async16(mine + d * THREADS, r.in + d * THREADS);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-    };
-    RowShare<DT, THREADS> now(a, blockIdx.x / C, RowFacts(a, p, blockIdx.x / C), rank, C);
-    RowFacts ahead(a, p, now.row + step);
-    first(now);
-    while (now.row < a.rows) {
-        const RowShare<DT, THREADS> next(a, now.row + step, ahead, rank, C);
-        ahead = RowFacts(a, p, now.row + 2 * step);
-        const T* x = static_cast<const T*>(a.data) + (uint64_t)now.row * a.row_stride;
-        float end = 0.0f, input = 0.0f;
-        if (now.end_at < a.vocab) end = E::up(x[now.end_at]);
-        if (tid == 32 && now.takes) input = E::up(x[now.y]);
-        Online o(c);
-        const uint4* in = now.in + kDepth * THREADS;
-        for (uint32_t j0 = 0; j0 < now.groups; j0 += kDepth) {
-#pragma unroll
-            for (int d = 0; d < kDepth; d++) {
-                if (j0 + d < now.groups) {
-                    asm volatile("cp.async.wait_group %0;" :: "n"(kDepth - 1) : "memory");
-                    o.add<DT>(mine[d * THREADS], c);
-                    if (j0 + d + kDepth < now.groups) copy_async16(mine + d * THREADS, in + d * THREADS);
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                }
+            if (j0 + d < now.groups) {
+                asm volatile("cp.async.wait_group %0;" :: "n"(kDepth - 1) : "memory");
+                o.add<DT>(mine[d * THREADS], c);
+                if (j0 + d + kDepth < now.groups) copy_async16(mine + d * THREADS, in + d * THREADS);
+                asm volatile("cp.async.commit_group;" ::: "memory");
             }
-            in += kDepth * THREADS;
         }
-        first(next);
-        if (now.takes) {
-            if (now.end_at < a.vocab) o.add(end, c);
-            if (tid == 32) z_y[n & 1] = input;
-            sums.give(o, n);
-            __syncthreads();
-            if (tid < 32) {
-                o = sums.take(c, n, rank, C);
-                if (tid == 0 && rank == 0) {
-                    const RowAnswer r = row_answer(o, z_y[n & 1], c);
-                    a.logp[now.row] = r.logp;
-                    if (a.lse) a.lse[now.row] = r.lse;
-                }
-            }
-            n++;
-        } else {
-            now.template skip<kModeLogprob>(a, rank, C);
+        in += kDepth * THREADS;
+    }
+    if (now.end_at < a.vocab) o.add(end, c);
+    sums.give(o, make_uint2(0u, 0u), 0, rank, C);
+    __syncthreads();
+    if (tid < 32) {
+        o = sums.take(c, 0, C);
+        if (tid == 0 && rank == 0) {
+            const RowAnswer r = row_answer(o, z_y, c);
+            a.logp[row] = r.logp;
+            if (a.lse) a.lse[row] = r.lse;
         }
-        now = next;
     }
     sums.finish(C);
 }
@@ -633,52 +682,83 @@ __device__ __forceinline__ double block_sum_d(double x, double* smem) {
     return s;
 }
 
+// What a part of the tokens makes of the record.
+struct PolicySums {
+    double l = 0.0, k = 0.0, w = 0.0;
+    uint32_t tokens = 0, clipped = 0;
+    float ratio = 0.0f;
+
+    __device__ __forceinline__ void add(const PolicySums& o) {
+        l += o.l;
+        k += o.k;
+        w += o.w;
+        tokens += o.tokens;
+        clipped += o.clipped;
+        ratio = fmaxf(ratio, o.ratio);
+    }
+    __device__ __forceinline__ void add_warp() {
+#pragma unroll
+        for (int mask = 16; mask >= 1; mask >>= 1) {
+            l += __shfl_xor_sync(0xFFFFFFFFu, l, mask);
+            k += __shfl_xor_sync(0xFFFFFFFFu, k, mask);
+            w += __shfl_xor_sync(0xFFFFFFFFu, w, mask);
+            ratio = fmaxf(ratio, __shfl_xor_sync(0xFFFFFFFFu, ratio, mask));
+        }
+        tokens = __reduce_add_sync(0xFFFFFFFFu, tokens);
+        clipped = __reduce_add_sync(0xFFFFFFFFu, clipped);
+    }
+};
+
 // Weighted sums of the policy loss over all tokens, and the gradient by log-probability.  `targets` (with vocab):
-// tokens whose target is out of range take no part.
+// tokens whose target is out of range take no part.  One cluster: its CTAs hand their sums to the first one, so the
+// record needs no scratch memory and no second launch.
 __global__ void __launch_bounds__(kVectorThreads)
 policy_kernel(const float* logp, uint64_t tokens, const int32_t* targets, uint32_t vocab, PolicyArgs p, float* coef,
               rlcu_policy_stat* stat, uint32_t flags) {
-    __shared__ double smem[kVectorThreads / 32];
-    double sum_l = 0.0, sum_k = 0.0, sum_w = 0.0, n = 0.0, cuts = 0.0;
-    float ratio = 0.0f;
-    for (uint64_t t = threadIdx.x; t < tokens; t += kVectorThreads) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    __shared__ PolicySums warps[kVectorThreads / 32], ctas[kMostCluster];
+    const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
+    PolicySums mine;
+    for (uint64_t t = rank * kVectorThreads + threadIdx.x; t < tokens; t += C * kVectorThreads) {
         const float w = p.weight[t];
         const bool takes = w != 0.0f && (!targets || (targets[t] >= 0 && (uint32_t)targets[t] < vocab));
         float co = 0.0f;
         if (takes) {
             const PolicyTerm o = policy_term(p, logp[t], t);
-            sum_l += (double)w * o.l;
-            sum_k += (double)w * o.k;
-            sum_w += w;
-            n += 1.0;
-            cuts += o.cut ? 1.0 : 0.0;
-            ratio = fmaxf(ratio, o.ratio);
+            mine.l += (double)w * o.l;
+            mine.k += (double)w * o.k;
+            mine.w += w;
+            mine.tokens++;
+            mine.clipped += o.cut;
+            mine.ratio = fmaxf(mine.ratio, o.ratio);
             co = o.coef;
         }
         if (coef) coef[t] = co;
     }
-    sum_l = block_sum_d(sum_l, smem);
-    sum_k = block_sum_d(sum_k, smem);
-    sum_w = block_sum_d(sum_w, smem);
-    n = block_sum_d(n, smem);
-    cuts = block_sum_d(cuts, smem);
-#pragma unroll
-    for (int mask = 16; mask >= 1; mask >>= 1) ratio = fmaxf(ratio, __shfl_xor_sync(0xFFFFFFFFu, ratio, mask));
+    mine.add_warp();
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = mine;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = ratio;
-    __syncthreads();
+    if (threadIdx.x < 32) {
+        mine = warps[threadIdx.x];
+        mine.add_warp();
+        if (threadIdx.x == 0) *cluster.map_shared_rank(&ctas[rank], 0) = mine;
+    }
+    cluster.sync();
+    if (rank != 0 || threadIdx.x >= 32) return;
+    mine = threadIdx.x < C ? ctas[threadIdx.x] : PolicySums();
+    mine.add_warp();
     if (threadIdx.x == 0) {
-        for (int w = 0; w < kVectorThreads / 32; w++) ratio = fmaxf(ratio, (float)smem[w]);
         rlcu_policy_stat r = {};
         if (flags & RLCU_LOSS_ACCUMULATE) r = *stat;
-        const double kl = p.hp.kl_coef != 0.0f ? (double)p.hp.kl_coef * sum_k : 0.0;
-        r.loss = (float)((double)r.loss + sum_l + kl);
-        r.policy = (float)((double)r.policy + sum_l);
-        r.kl = (float)((double)r.kl + sum_k);
-        r.weight = (float)((double)r.weight + sum_w);
-        r.tokens += (uint32_t)n;
-        r.clipped += (uint32_t)cuts;
-        r.ratio_max = fmaxf(r.ratio_max, ratio);
+        const double kl = p.hp.kl_coef != 0.0f ? (double)p.hp.kl_coef * mine.k : 0.0;
+        r.loss = (float)((double)r.loss + mine.l + kl);
+        r.policy = (float)((double)r.policy + mine.l);
+        r.kl = (float)((double)r.kl + mine.k);
+        r.weight = (float)((double)r.weight + mine.w);
+        r.tokens += mine.tokens;
+        r.clipped += mine.clipped;
+        r.ratio_max = fmaxf(r.ratio_max, mine.ratio);
         *stat = r;
     }
 }
@@ -852,11 +932,8 @@ int launch_rows(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, const 
     return RLCU_OK;
 }
 
-template <typename Kernel>
-int launch_clusters(Kernel kernel, const LogitsArgs& a, const PolicyArgs& p, int cluster, int threads, int smem, cudaStream_t s) {
-    RLCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (cluster > 8) RLCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    cudaLaunchAttribute attr[1];
+// one cluster of `cluster` CTAs
+cudaLaunchConfig_t cluster_launch(cudaLaunchAttribute* attr, int cluster, int threads, int smem, cudaStream_t s) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -867,13 +944,16 @@ int launch_clusters(Kernel kernel, const LogitsArgs& a, const PolicyArgs& p, int
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    int most = 0;
-    RLCU_CUDA(cudaOccupancyMaxActiveClusters(&most, kernel, &cfg));
-    if (most < 1) return set_error(RLCU_ERR_CUDA, "kernel does not fit on an SM");
-#ifdef EACH
-    if (smem == 0) most = 1 << 24;
-#endif
-    cfg.gridDim = dim3((unsigned)((a.rows < (uint64_t)most ? a.rows : (uint64_t)most) * cluster));
+    return cfg;
+}
+
+template <typename Kernel>
+int launch_clusters(Kernel kernel, const LogitsArgs& a, const PolicyArgs& p, int cluster, int threads, int smem, cudaStream_t s) {
+    RLCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (cluster > 8) RLCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = cluster_launch(attr, cluster, threads, smem, s);
+    cfg.gridDim = dim3((unsigned)(a.rows * cluster));
     RLCU_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, p));
     return RLCU_OK;
 }
@@ -918,7 +998,7 @@ int launch_logits(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, cuda
     const bool alike = MODE != kModePolicy || (((reinterpret_cast<uintptr_t>(a.grad) ^ reinterpret_cast<uintptr_t>(a.data)) & 15) == 0 &&
                                                (a.grad_stride - a.row_stride) * esz % 16 == 0);
     const bool fits = MODE != kModePolicy || groups <= (uint64_t)kMostCluster * kWide * kMostHeld;
-    if (!alike || !fits || groups < 64) return launch_rows<MODE>(a, p, dtype, nullptr, nullptr, s);
+    if (!alike || !fits || groups < 64 || a.rows > 0x7FFFFFFFull / kMostCluster) return launch_rows<MODE>(a, p, dtype, nullptr, nullptr, s);
     if (dtype == RLCU_F16) return launch_logits_dt<RLCU_F16, MODE>(a, p, sms, groups, s);
     if (dtype == RLCU_BF16) return launch_logits_dt<RLCU_BF16, MODE>(a, p, sms, groups, s);
     return launch_logits_dt<RLCU_F32, MODE>(a, p, sms, groups, s);
@@ -926,8 +1006,9 @@ int launch_logits(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, cuda
 
 int launch_policy(const float* logp, uint64_t tokens, const int32_t* targets, uint32_t vocab, const PolicyArgs& p,
                   float* coef, rlcu_policy_stat* stat, uint32_t flags, cudaStream_t s) {
-    policy_kernel<<<1, kVectorThreads, 0, s>>>(logp, tokens, targets, vocab, p, coef, stat, flags);
-    RLCU_CUDA(cudaGetLastError());
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = cluster_launch(attr, tokens <= kVectorThreads ? 1 : tokens <= 4 * kVectorThreads ? 4 : 8, kVectorThreads, 0, s);
+    RLCU_CUDA(cudaLaunchKernelEx(&cfg, policy_kernel, logp, tokens, targets, vocab, p, coef, stat, flags));
     return RLCU_OK;
 }
 
