@@ -26,6 +26,12 @@ constexpr float kLog2E = 1.4426950408889634f;
 #ifndef HELD_CTAS
 #define HELD_CTAS (1024 / THREADS)
 #endif
+#ifndef PREF_C
+#define PREF_C 16
+#endif
+#ifndef POL_C
+#define POL_C 8
+#endif
 #ifndef SUM_DEPTH
 #define SUM_DEPTH 4
 #endif
@@ -665,22 +671,61 @@ logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
     sums.finish(C);
 }
 
+// The gradient alone (the sum is known): elementwise, a CTA per run of kGradGroups groups of a row, so that the grid
+// moves through memory in order.
+constexpr int kGradThreads = 256, kGradPer = 4, kGradGroups = kGradThreads * kGradPer;
+
+template <uint32_t DT>
+__global__ void __launch_bounds__(kGradThreads)
+logits_grad_kernel(LogitsArgs a, const float* lse_in, const float* coef_in, uint32_t runs) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    const uint32_t row = blockIdx.x / runs, run = blockIdx.x - row * runs;
+    const uint32_t tid = threadIdx.x;
+    const int32_t y = a.targets[row];
+    const float coef = coef_in[row], lse = lse_in[row], S = a.scaler ? a.scaler->scale : 1.0f;
+    const T* x = static_cast<const T*>(a.data) + (uint64_t)row * a.row_stride;
+    T* g = static_cast<T*>(a.grad) + (uint64_t)row * a.grad_stride;
+    const RowCut cut = cut_row(x, a.vocab);
+    const uint32_t tail = cut.head + cut.groups * E::kVec, ends = cut.head + (a.vocab - tail);
+    const uint32_t end_at = tid < cut.head ? tid : tail + (tid - cut.head);
+    const bool has_end = run == 0 && tid < ends, takes = y >= 0 && (uint32_t)y < a.vocab && coef != 0.0f;
+    const uint4* in = reinterpret_cast<const uint4*>(x + cut.head);
+    uint4* out = reinterpret_cast<uint4*>(g + cut.head);
+    const uint32_t lo = run * kGradGroups + tid;
+    if (!takes) {
+#pragma unroll
+        for (int j = 0; j < kGradPer; j++)
+            if (lo + j * kGradThreads < cut.groups) __stcs(out + lo + j * kGradThreads, make_uint4(0u, 0u, 0u, 0u));
+        if (has_end) g[end_at] = E::down(0.0f);
+        return;
+    }
+    uint4 v[kGradPer];
+#pragma unroll
+    for (int j = 0; j < kGradPer; j++)
+        if (lo + j * kGradThreads < cut.groups) v[j] = __ldcs(in + lo + j * kGradThreads);
+    const float c = a.inv_temperature * kLog2E, k = coef * S * a.inv_temperature;
+    // 2^(c z - log2e lse) = 2^(c z - e) * 2^(e - log2e lse), e an integer
+    const bool empty = lse == -INFINITY;
+    const float e = empty ? 0.0f : rintf(lse * kLog2E), kn = empty ? 0.0f * k : -k * exp2f(-fmaf(lse, kLog2E, -e));
+    // the target's logit is read by the thread that overwrites it
+    const uint32_t group = ((uint32_t)y - cut.head) / E::kVec;
+    const bool in_groups = (uint32_t)y >= cut.head && (uint32_t)y < tail;
+    const bool owns_y = in_groups ? group / kGradGroups == run && group % kGradThreads == tid : has_end && end_at == (uint32_t)y;
+    float ky = 0.0f;
+    if (owns_y) ky = empty ? k : -k * expm1f(fmaf(E::up(x[y]), a.inv_temperature, -lse));
+    if (has_end) g[end_at] = E::down(kn * exp2_fast(fmaf(E::up(x[end_at]), c, -e)));
+#pragma unroll
+    for (int j = 0; j < kGradPer; j++)
+        if (lo + j * kGradThreads < cut.groups) __stcs(out + lo + j * kGradThreads, grad_group<DT>(v[j], c, e, kn));
+    if (owns_y) g[y] = E::down(ky);
+}
+
 // ---------------------------------------------------------------------------
 // policy loss of log-probabilities
 // ---------------------------------------------------------------------------
 
 constexpr int kVectorThreads = 1024;
-
-__device__ __forceinline__ double block_sum_d(double x, double* smem) {
-#pragma unroll
-    for (int mask = 16; mask >= 1; mask >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, mask);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = x;
-    __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < (int)(blockDim.x >> 5); w++) s += smem[w];
-    return s;
-}
 
 // What a part of the tokens makes of the record.
 struct PolicySums {
@@ -807,55 +852,160 @@ __device__ __forceinline__ void preference_term(const rlcu_preference_hparams& h
     slope *= beta;
 }
 
+// One cluster, so that the record needs no scratch memory and no second launch.  CTA r has the pairs r, r + C, ... and
+// works on kBatch of them at a time, whatever their lengths: their tokens are cut into at most kSegments segments of
+// equal length, a warp sums a segment, and the segments of a sequence are added in order.
+constexpr int kBatch = 16, kSegments = 512;
+
 __global__ void __launch_bounds__(kVectorThreads)
 preference_kernel(PreferenceArgs a) {
-    __shared__ double smem[kVectorThreads / 32];
-    double loss_sum = 0.0, margin_sum = 0.0;
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    constexpr int kWarps = kVectorThreads / 32;
+    __shared__ uint32_t begin[2 * kBatch], length[2 * kBatch], first_segment[2 * kBatch + 1], segment;
+    __shared__ double part[kSegments + 2 * kBatch], sums[2 * kBatch];
+    __shared__ uint32_t counted[kSegments + 2 * kBatch], counts[2 * kBatch];
+    __shared__ float coefs[2 * kBatch];
+    __shared__ double totals[kMostCluster][2];
+    __shared__ uint32_t corrects[kMostCluster];
+    const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    double loss_sum = 0.0, margin_sum = 0.0;          // of threads 0 to kBatch - 1
     uint32_t correct = 0;
-    const uint64_t first = offset_at(a, 0);
-    if (a.coef)
-        for (uint64_t t = threadIdx.x; t < first; t += kVectorThreads) a.coef[t] = 0.0f;
-    uint64_t lo = first;
-    for (uint64_t i = 0; i < a.pairs; i++) {
-        double s[2], share[2];
-        uint64_t at[3] = {lo, 0, 0};
-        for (int q = 0; q < 2; q++) {
-            at[q + 1] = offset_at(a, 2 * i + q + 1);
-            if (at[q + 1] < at[q]) at[q + 1] = at[q];
-            double sum = 0.0, n = 0.0;
-            for (uint64_t t = at[q] + threadIdx.x; t < at[q + 1]; t += kVectorThreads) {
-                if (a.mask && !a.mask[t]) continue;
-                sum += (double)(a.ref_logp ? a.logp[t] - a.ref_logp[t] : a.logp[t]);
-                n += 1.0;
+
+    for (uint64_t base = 0; base * C + rank < a.pairs; base += kBatch) {
+        if (warp == 0) {
+            // lane q: sequence q of the batch
+            static_assert(2 * kBatch == 32, "a lane per sequence");
+            const uint64_t pair = (base + lane / 2) * C + rank;
+            uint32_t lo = 0, n = 0;
+            if (pair < a.pairs) {
+                const uint64_t chosen = offset_at(a, 2 * pair), rejected = max(chosen, offset_at(a, 2 * pair + 1));
+                const uint64_t behind = max(rejected, offset_at(a, 2 * pair + 2));
+                lo = (uint32_t)(lane & 1 ? rejected : chosen);
+                n = (uint32_t)(lane & 1 ? behind : rejected) - lo;
             }
-            s[q] = block_sum_d(sum, smem);
-            n = a.hp.length_mean ? block_sum_d(n, smem) : 1.0;
-            share[q] = n > 0.0 ? 1.0 / n : 0.0;
-            s[q] *= share[q];
+            unsigned long long all = n;
+#pragma unroll
+            for (int mask = 16; mask >= 1; mask >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, mask);
+            const uint32_t seg = max(256u, (uint32_t)((all + kSegments - 1) / kSegments));
+            uint32_t before = (n + seg - 1) / seg;
+            const uint32_t own = before;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t left = __shfl_up_sync(0xFFFFFFFFu, before, d);
+                if ((int)lane >= d) before += left;
+            }
+            begin[lane] = lo;
+            length[lane] = n;
+            first_segment[lane] = before - own;
+            if (lane == 31) first_segment[32] = before;
+            if (lane == 0) segment = seg;
         }
-        double h, loss, slope;
-        preference_term(a.hp, s[0], s[1], h, loss, slope);
-        const double w = a.pair_weight ? (double)a.pair_weight[i] : 1.0 / (double)a.pairs;
-        loss_sum += w * loss;
-        margin_sum += w * h;
-        correct += s[0] > s[1];
-        if (threadIdx.x == 0 && a.rewards) {
-            a.rewards[2 * i] = (float)((double)a.hp.beta * s[0]);
-            a.rewards[2 * i + 1] = (float)((double)a.hp.beta * s[1]);
+        __syncthreads();
+        const uint32_t segments = first_segment[2 * kBatch], seg = segment;
+        for (uint32_t s = warp; s < segments; s += kWarps) {
+            const uint32_t q = 31 - __clz(__ballot_sync(0xFFFFFFFFu, first_segment[lane] <= s));      // last sequence that begins by s
+            const uint32_t at = (s - first_segment[q]) * seg, hi = min(at + seg, length[q]);
+            const uint32_t t0 = begin[q];
+            double sum = 0.0;
+            uint32_t n = 0;
+#pragma unroll 8
+            for (uint32_t t = at + lane; t < hi; t += 32) {
+                const float ref = a.ref_logp ? a.ref_logp[t0 + t] : 0.0f, lp = a.logp[t0 + t];
+                const bool counts_here = !a.mask || a.mask[t0 + t];
+                if (counts_here) {
+                    sum += (double)(lp - ref);
+                    n++;
+                }
+            }
+#pragma unroll
+            for (int mask = 16; mask >= 1; mask >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, mask);
+            n = __reduce_add_sync(0xFFFFFFFFu, n);
+            if (lane == 0) {
+                part[s] = sum;
+                counted[s] = n;
+            }
         }
-        if (a.coef)
+        __syncthreads();
+        for (uint32_t q = warp; q < 2 * kBatch; q += kWarps) {
+            double sum = 0.0;
+            uint32_t n = 0;
+            for (uint32_t s = first_segment[q] + lane; s < first_segment[q + 1]; s += 32) {
+                sum += part[s];
+                n += counted[s];
+            }
+#pragma unroll
+            for (int mask = 16; mask >= 1; mask >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, mask);
+            n = __reduce_add_sync(0xFFFFFFFFu, n);
+            if (lane == 0) {
+                sums[q] = sum;
+                counts[q] = n;
+            }
+        }
+        __syncthreads();
+        const uint64_t pair = (base + tid) * C + rank;
+        if (tid < kBatch && pair < a.pairs) {
+            double s[2], share[2];
             for (int q = 0; q < 2; q++) {
-                const float co = (float)((q ? -slope : slope) * w * share[q]);
-                for (uint64_t t = at[q] + threadIdx.x; t < at[q + 1]; t += kVectorThreads)
-                    a.coef[t] = !a.mask || a.mask[t] ? co : 0.0f;
+                share[q] = a.hp.length_mean ? (counts[2 * tid + q] ? 1.0 / counts[2 * tid + q] : 0.0) : 1.0;
+                s[q] = sums[2 * tid + q] * share[q];
             }
-        lo = at[2];
+            double h, loss, slope;
+            preference_term(a.hp, s[0], s[1], h, loss, slope);
+            const double w = a.pair_weight ? (double)a.pair_weight[pair] : 1.0 / (double)a.pairs;
+            loss_sum += w * loss;
+            margin_sum += w * h;
+            correct += s[0] > s[1];
+            for (int q = 0; q < 2; q++) {
+                if (a.rewards) a.rewards[2 * pair + q] = (float)((double)a.hp.beta * s[q]);
+                coefs[2 * tid + q] = (float)((q ? -slope : slope) * w * share[q]);
+            }
+        }
+        __syncthreads();
+        if (a.coef)
+            for (uint32_t s = warp; s < segments; s += kWarps) {
+                const uint32_t q = 31 - __clz(__ballot_sync(0xFFFFFFFFu, first_segment[lane] <= s));
+                const uint32_t at = (s - first_segment[q]) * seg, hi = min(at + seg, length[q]);
+                const uint32_t t0 = begin[q];
+                const float co = coefs[q];
+#pragma unroll 8
+                for (uint32_t t = at + lane; t < hi; t += 32) a.coef[t0 + t] = !a.mask || a.mask[t0 + t] ? co : 0.0f;
+            }
+        __syncthreads();                              // the batch's tables are written again
     }
-    if (a.coef)
-        for (uint64_t t = lo + threadIdx.x; t < a.tokens; t += kVectorThreads) a.coef[t] = 0.0f;
-    if (threadIdx.x == 0) {
+    if (a.coef) {
+        // tokens of no sequence
+        const uint64_t first = offset_at(a, 0);
+        uint64_t behind = first;
+        if (a.pairs) behind = max(max(offset_at(a, 2 * a.pairs - 2), offset_at(a, 2 * a.pairs - 1)), offset_at(a, 2 * a.pairs));
+        for (uint64_t t = rank * kVectorThreads + tid; t < first; t += C * kVectorThreads) a.coef[t] = 0.0f;
+        for (uint64_t t = behind + rank * kVectorThreads + tid; t < a.tokens; t += C * kVectorThreads) a.coef[t] = 0.0f;
+    }
+    if (warp == 0) {
+#pragma unroll
+        for (int mask = 16; mask >= 1; mask >>= 1) {
+            loss_sum += __shfl_xor_sync(0xFFFFFFFFu, loss_sum, mask);
+            margin_sum += __shfl_xor_sync(0xFFFFFFFFu, margin_sum, mask);
+        }
+        correct = __reduce_add_sync(0xFFFFFFFFu, correct);
+        if (lane == 0) {
+            *cluster.map_shared_rank(&totals[rank][0], 0) = loss_sum;
+            *cluster.map_shared_rank(&totals[rank][1], 0) = margin_sum;
+            *cluster.map_shared_rank(&corrects[rank], 0) = correct;
+        }
+    }
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
         rlcu_preference_stat r = {};
         if (a.flags & RLCU_LOSS_ACCUMULATE) r = *a.stat;
+        loss_sum = margin_sum = 0.0;
+        correct = 0;
+        for (uint32_t i = 0; i < C; i++) {
+            loss_sum += totals[i][0];
+            margin_sum += totals[i][1];
+            correct += corrects[i];
+        }
         r.loss = (float)((double)r.loss + loss_sum);
         r.margin = (float)((double)r.margin + margin_sum);
         r.pairs += (uint32_t)a.pairs;
@@ -988,26 +1138,41 @@ int launch_logits_dt(const LogitsArgs& a, const PolicyArgs& p, int sms, uint64_t
                           : launch_clusters(logits_sum_kernel<DT, kNarrow>, a, p, cluster, kNarrow, kDepth * kNarrow * 16, s);
 }
 
+// every row of the gradient starts at the same place of a 16-byte group as its logits do
+bool alike(const LogitsArgs& a, size_t esz) {
+    return ((reinterpret_cast<uintptr_t>(a.grad) ^ reinterpret_cast<uintptr_t>(a.data)) & 15) == 0 && (a.grad_stride - a.row_stride) * esz % 16 == 0;
+}
+
 template <int MODE>
 int launch_logits(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, cudaStream_t s) {
     int sms = 0;
     if (const int rc = sm_count(&sms)) return rc;
     const size_t esz = dtype_bytes(dtype);
     const uint64_t groups = a.vocab / (16 / esz);
-    // every row of the gradient starts at the same place of a 16-byte group as its logits do
-    const bool alike = MODE != kModePolicy || (((reinterpret_cast<uintptr_t>(a.grad) ^ reinterpret_cast<uintptr_t>(a.data)) & 15) == 0 &&
-                                               (a.grad_stride - a.row_stride) * esz % 16 == 0);
     const bool fits = MODE != kModePolicy || groups <= (uint64_t)kMostCluster * kWide * kMostHeld;
-    if (!alike || !fits || groups < 64 || a.rows > 0x7FFFFFFFull / kMostCluster) return launch_rows<MODE>(a, p, dtype, nullptr, nullptr, s);
+    if ((MODE == kModePolicy && !alike(a, esz)) || !fits || groups < 64 || a.rows > 0x7FFFFFFFull / kMostCluster) return launch_rows<MODE>(a, p, dtype, nullptr, nullptr, s);
     if (dtype == RLCU_F16) return launch_logits_dt<RLCU_F16, MODE>(a, p, sms, groups, s);
     if (dtype == RLCU_BF16) return launch_logits_dt<RLCU_BF16, MODE>(a, p, sms, groups, s);
     return launch_logits_dt<RLCU_F32, MODE>(a, p, sms, groups, s);
 }
 
+int launch_grad(const LogitsArgs& a, uint32_t dtype, const float* lse, const float* coef, cudaStream_t s) {
+    const size_t esz = dtype_bytes(dtype);
+    const uint64_t groups = a.vocab / (16 / esz), runs = (groups + kGradGroups - 1) / kGradGroups;
+    if (!alike(a, esz) || groups < 64 || a.rows * runs > 0x7FFFFFFFull) return launch_rows<kModeGrad>(a, PolicyArgs{}, dtype, lse, coef, s);
+    const unsigned grid = (unsigned)(a.rows * runs);
+    if (dtype == RLCU_F16) logits_grad_kernel<RLCU_F16><<<grid, kGradThreads, 0, s>>>(a, lse, coef, (uint32_t)runs);
+    else if (dtype == RLCU_BF16) logits_grad_kernel<RLCU_BF16><<<grid, kGradThreads, 0, s>>>(a, lse, coef, (uint32_t)runs);
+    else logits_grad_kernel<RLCU_F32><<<grid, kGradThreads, 0, s>>>(a, lse, coef, (uint32_t)runs);
+    RLCU_CUDA(cudaGetLastError());
+    return RLCU_OK;
+}
+
 int launch_policy(const float* logp, uint64_t tokens, const int32_t* targets, uint32_t vocab, const PolicyArgs& p,
                   float* coef, rlcu_policy_stat* stat, uint32_t flags, cudaStream_t s) {
+    if (POL_C > 8) RLCU_CUDA(cudaFuncSetAttribute(policy_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = cluster_launch(attr, tokens <= kVectorThreads ? 1 : tokens <= 4 * kVectorThreads ? 4 : 8, kVectorThreads, 0, s);
+    cudaLaunchConfig_t cfg = cluster_launch(attr, tokens <= kVectorThreads ? 1 : tokens <= 4 * kVectorThreads ? 4 : POL_C, kVectorThreads, 0, s);
     RLCU_CUDA(cudaLaunchKernelEx(&cfg, policy_kernel, logp, tokens, targets, vocab, p, coef, stat, flags));
     return RLCU_OK;
 }
@@ -1035,7 +1200,7 @@ extern "C" int rlcu_token_logprob_grad(const void* logits, uint32_t dtype, uint6
     if (rows && (!lse || !coef)) return set_error(RLCU_ERR_INVALID, "null lse or coef");
     if (!rows) return RLCU_OK;
     LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, nullptr, nullptr, grad, grad_stride, scaler};
-    return launch_rows<kModeGrad>(a, PolicyArgs{}, dtype, lse, coef, (cudaStream_t)stream);
+    return launch_grad(a, dtype, lse, coef, (cudaStream_t)stream);
 }
 
 extern "C" int rlcu_policy_loss_logp(const float* logp, uint64_t tokens, const float* old_logp, const float* ref_logp,
@@ -1084,7 +1249,12 @@ extern "C" int rlcu_preference_loss(const float* logp, uint64_t tokens, const fl
     if (!offsets) return set_error(RLCU_ERR_INVALID, "null offsets");
     if (tokens && !logp) return set_error(RLCU_ERR_INVALID, "null logp");
     PreferenceArgs a = {logp, ref_logp, mask, offsets, pair_weight, tokens, pairs, *hp, coef, rewards, stat, flags};
-    preference_kernel<<<1, kVectorThreads, 0, (cudaStream_t)stream>>>(a);
-    RLCU_CUDA(cudaGetLastError());
+    // more CTAs than pairs would idle; below a few thousand tokens each, the cluster costs more than it saves
+    int cluster = 1;
+    while (cluster < PREF_C && (uint64_t)cluster < pairs && tokens > (uint64_t)cluster * 4096) cluster *= 2;
+    if (cluster > 8) RLCU_CUDA(cudaFuncSetAttribute(preference_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = cluster_launch(attr, cluster, kVectorThreads, 0, (cudaStream_t)stream);
+    RLCU_CUDA(cudaLaunchKernelEx(&cfg, preference_kernel, a));
     return RLCU_OK;
 }
