@@ -12,6 +12,12 @@
 #include "host_util.h"
 #include "typed.cuh"
 
+#ifndef GRAD_CTAS
+#define GRAD_CTAS (512 / THREADS)
+#endif
+#ifndef GRAD_PARTS
+#define GRAD_PARTS 296
+#endif
 namespace rlcu {
 namespace {
 
@@ -104,6 +110,219 @@ act8_load_kernel(const uint8_t* codes, uint64_t code_stride, const uint8_t* scal
             const uint32_t j = col + i * 32 + lane;
             if (j < cols) out[j] = E::down(keep_finite<DT>(decode(codes[row * code_stride + j], scale)));
         }
+    }
+}
+
+// The same in 16-byte accesses, for rows that start on 16-byte boundaries: eight threads per block of 128, 16 columns
+// each (one 16-byte group of codes).  Pure streaming; a CTA takes kVecBlocks consecutive blocks.
+constexpr int kRun = 16;                                   // columns per thread and step
+constexpr int kVecSteps = 2;
+constexpr uint32_t kVecBlocks = kAct8Threads / (kBlock / kRun) * kVecSteps;
+
+// 32 bytes in one access where the address allows it (sm_100): a thread's 16 columns of 16 bits
+__device__ __forceinline__ void load32(const void* p, uint4& a, uint4& b) {
+    if ((reinterpret_cast<uintptr_t>(p) & 31u) == 0) {
+        asm volatile("ld.global.cs.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
+    } else {
+        a = __ldcs(static_cast<const uint4*>(p));
+        b = __ldcs(static_cast<const uint4*>(p) + 1);
+    }
+}
+__device__ __forceinline__ void store32(void* p, uint4 a, uint4 b) {
+    if ((reinterpret_cast<uintptr_t>(p) & 31u) == 0) {
+        asm volatile("st.global.cs.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                     :: "l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+    } else {
+        __stcs(static_cast<uint4*>(p), a);
+        __stcs(static_cast<uint4*>(p) + 1, b);
+    }
+}
+
+// 16 columns as they are in memory
+template <uint32_t DT>
+struct Run {
+    static constexpr int kGroups = kRun / Elem<DT>::kVec;
+    uint4 v[kGroups];
+
+    __device__ __forceinline__ void load(const void* p) {
+#pragma unroll
+        for (int i = 0; i < kGroups; i += 2) load32(static_cast<const uint4*>(p) + i, v[i], v[i + 1]);
+    }
+    __device__ __forceinline__ void store(void* p) const {
+#pragma unroll
+        for (int i = 0; i < kGroups; i += 2) store32(static_cast<uint4*>(p) + i, v[i], v[i + 1]);
+    }
+    // the first n of them, one by one
+    __device__ __forceinline__ void load_part(const typename Elem<DT>::T* p, int n) {
+        float f[kRun];
+#pragma unroll
+        for (int i = 0; i < kRun; i++) f[i] = i < n ? Elem<DT>::up(p[i]) : 0.0f;
+        set(f);
+    }
+    __device__ __forceinline__ void store_part(typename Elem<DT>::T* p, int n) const {
+        float f[kRun];
+        get(f);
+#pragma unroll
+        for (int i = 0; i < kRun; i++)
+            if (i < n) p[i] = Elem<DT>::down(f[i]);
+    }
+    __device__ __forceinline__ void get(float (&f)[kRun]) const {
+#pragma unroll
+        for (int i = 0; i < kGroups; i++) {
+            float g[Elem<DT>::kVec];
+            Elem<DT>::unpack(v[i], g);
+#pragma unroll
+            for (int q = 0; q < Elem<DT>::kVec; q++) f[i * Elem<DT>::kVec + q] = g[q];
+        }
+    }
+    __device__ __forceinline__ void set(const float (&f)[kRun]) {
+#pragma unroll
+        for (int i = 0; i < kGroups; i++) {
+            float g[Elem<DT>::kVec];
+#pragma unroll
+            for (int q = 0; q < Elem<DT>::kVec; q++) g[q] = f[i * Elem<DT>::kVec + q];
+            v[i] = Elem<DT>::pack(g);
+        }
+    }
+};
+// the codes of 16 columns, the first n of them where the row ends sooner
+__device__ __forceinline__ uint4 load_codes(const uint8_t* p, int n) {
+    if (n >= kRun) return __ldcs(reinterpret_cast<const uint4*>(p));
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kRun; i++)
+        if (i < n) w[i / 4] |= (uint32_t)p[i] << (i % 4 * 8);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// four codes of finite values (or NaN)
+__device__ __forceinline__ uint32_t encode4(const float* q) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(q[1]), "f"(q[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(q[3]), "f"(q[2]));
+    return (uint32_t)lo | (uint32_t)hi << 16;
+}
+__device__ __forceinline__ void decode4(uint32_t w, float* f) {
+    uint32_t a, b;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"((uint16_t)w));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"((uint16_t)(w >> 16)));
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    f[0] = x.x;
+    f[1] = x.y;
+    f[2] = y.x;
+    f[3] = y.y;
+}
+// 16 codes as values, before any rounding; finite ones stay finite
+__device__ __forceinline__ void decode_run(uint4 v, uint32_t byte, float (&f)[kRun]) {
+    decode4(v.x, f);
+    decode4(v.y, f + 4);
+    decode4(v.z, f + 8);
+    decode4(v.w, f + 12);
+    const float scale = pow2((int)byte - 127);
+#pragma unroll
+    for (int i = 0; i < kRun; i++) f[i] *= scale;
+    if (byte >= 127 + 119) {                               // 448 * 2^119 < 2^128
+#pragma unroll
+        for (int i = 0; i < kRun; i++) f[i] = fabsf(f[i]) > FLT_MAX ? copysignf(FLT_MAX, f[i]) : f[i];
+    }
+}
+// where a thread's step k of a CTA's blocks lies
+struct Place {
+    uint32_t block, row, col;
+    int n;                       // columns of its 16 that the row has
+
+    __device__ __forceinline__ Place(int k, uint32_t total, uint32_t blocks, uint32_t cols) {
+        block = blockIdx.x * kVecBlocks + k * (kVecBlocks / kVecSteps) + threadIdx.x / (kBlock / kRun);
+        row = block / blocks;
+        col = (block - row * blocks) * kBlock + threadIdx.x % (kBlock / kRun) * kRun;
+        n = block < total ? (int)cols - (int)col : 0;
+    }
+};
+
+template <uint32_t DT>
+__global__ void __launch_bounds__(kAct8Threads)
+act8_store_vec_kernel(const void* x, uint32_t total, uint32_t blocks, uint32_t cols, uint64_t x_stride, uint8_t* codes,
+                      uint64_t code_stride, uint8_t* scales) {
+    using T = typename Elem<DT>::T;
+    Run<DT> runs[kVecSteps];
+#pragma unroll
+    for (int k = 0; k < kVecSteps; k++) {
+        const Place at(k, total, blocks, cols);
+        const T* in = static_cast<const T*>(x) + at.row * x_stride + at.col;
+        if (at.n >= kRun) runs[k].load(in);
+        else runs[k].load_part(in, at.n);
+    }
+#pragma unroll
+    for (int k = 0; k < kVecSteps; k++) {
+        const Place at(k, total, blocks, cols);
+        float f[kRun], top = 0.0f;
+        runs[k].get(f);
+#pragma unroll
+        for (int i = 0; i < kRun; i++) top = fmaxf(top, fabsf(f[i]));             // NaN is passed over
+#pragma unroll
+        for (int mask = 4; mask >= 1; mask >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, mask));
+        if (__any_sync(0xFFFFFFFFu, top > FLT_MAX)) {                              // an infinity somewhere: finite values count
+            top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                if (fabsf(f[i]) <= FLT_MAX) top = fmaxf(top, fabsf(f[i]));
+                else f[i] = NAN;
+            }
+#pragma unroll
+            for (int mask = 4; mask >= 1; mask >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, mask));
+        }
+        if (at.n <= 0) {
+            // (a block's last threads may have no column; the first one has)
+            continue;
+        }
+        const uint32_t byte = scale_byte(top);
+        const float inv = pow2(127 - (int)byte);
+#pragma unroll
+        for (int i = 0; i < kRun; i++) f[i] *= inv;
+        const uint4 q = make_uint4(encode4(f), encode4(f + 4), encode4(f + 8), encode4(f + 12));
+        uint8_t* out = codes + at.row * code_stride + at.col;
+        if (at.n >= kRun) {
+            *reinterpret_cast<uint4*>(out) = q;
+        } else {
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < kRun; i++)
+                if (i < at.n) out[i] = (uint8_t)(w[i / 4] >> (i % 4 * 8));
+        }
+        if (threadIdx.x % (kBlock / kRun) == 0) scales[at.block] = (uint8_t)byte;
+    }
+}
+
+template <uint32_t DT>
+__global__ void __launch_bounds__(kAct8Threads)
+act8_load_vec_kernel(const uint8_t* codes, uint64_t code_stride, const uint8_t* scales, uint32_t total, uint32_t blocks,
+                     uint32_t cols, void* x, uint64_t x_stride) {
+    using T = typename Elem<DT>::T;
+    uint4 v[kVecSteps];
+    uint32_t byte[kVecSteps];
+#pragma unroll
+    for (int k = 0; k < kVecSteps; k++) {
+        const Place at(k, total, blocks, cols);
+        if (at.n > 0) {
+            v[k] = load_codes(codes + at.row * code_stride + at.col, at.n);
+            byte[k] = scales[at.block];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kVecSteps; k++) {
+        const Place at(k, total, blocks, cols);
+        if (at.n <= 0) continue;
+        float f[kRun];
+        decode_run(v[k], byte[k], f);
+        if (DT == RLCU_F16 ? byte[k] >= 127 + 7 : DT == RLCU_BF16 && byte[k] >= 127 + 119) {      // 448 * 2^7 < 65504
+#pragma unroll
+            for (int i = 0; i < kRun; i++) f[i] = keep_finite<DT>(f[i]);
+        }
+        Run<DT> run;
+        run.set(f);
+        T* out = static_cast<T*>(x) + at.row * x_stride + at.col;
+        if (at.n >= kRun) run.store(out);
+        else run.store_part(out, at.n);
     }
 }
 
@@ -211,11 +430,216 @@ norm_grad_kernel(NormArgs a) {
     }
 }
 
+// Rows that start on 16-byte boundaries: TPR threads per row, each with the same NV runs of 16 columns of every row it
+// works on (so their weights stay in registers), a CTA with THREADS / TPR rows at a time.  The row is decoded once; the
+// sums over it go through one barrier (none where a warp has the row).
+template <int TPR, int THREADS>
+struct RowSum {
+    float2 part[2][THREADS / 32];              // by step parity
+    __device__ __forceinline__ float2 operator()(float x, float y, uint32_t step) {
+#pragma unroll
+        for (int mask = 16; mask >= 1; mask >>= 1) {
+            x += __shfl_xor_sync(0xFFFFFFFFu, x, mask);
+            y += __shfl_xor_sync(0xFFFFFFFFu, y, mask);
+        }
+        if (TPR == 32) return make_float2(x, y);
+        static_assert(TPR == 32 || TPR == THREADS, "a warp or a CTA per row");
+        if ((threadIdx.x & 31) == 0) part[step & 1][threadIdx.x >> 5] = make_float2(x, y);
+        __syncthreads();
+        x = y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; w++) {
+            x += part[step & 1][w].x;
+            y += part[step & 1][w].y;
+        }
+        return make_float2(x, y);
+    }
+};
+
+template <int TPR, int NV>
+__device__ __forceinline__ void load_weights(const NormArgs& a, float (&w)[NV][kRun]) {
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int i = 0; i < kRun; i++) {
+            const uint32_t j = (k * TPR + threadIdx.x % TPR) * kRun + i;
+            w[k][i] = j < a.cols ? weight_at(a, j) : 0.0f;
+        }
+}
+
+template <uint32_t DT, int TPR, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+norm_vec_kernel(NormArgs a, uint32_t rows_per_cta) {
+    using T = typename Elem<DT>::T;
+    __shared__ RowSum<TPR, THREADS> sum;
+    const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows;
+    const uint32_t first = blockIdx.x * rows_per_cta + threadIdx.x / TPR, last = min(rows, (blockIdx.x + 1) * rows_per_cta);
+    float w[NV][kRun];
+    load_weights<TPR, NV>(a, w);
+    uint32_t step = 0;
+    for (uint32_t row = first; row < last; row += THREADS / TPR, step++) {
+        float v[NV][kRun], sq = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const uint32_t col = (k * TPR + lane) * kRun;
+            if (col < a.cols) {
+                decode_run(load_codes(a.codes + row * a.code_stride + col, (int)a.cols - (int)col), a.scales[(uint64_t)row * a.blocks + col / kBlock], v[k]);
+#pragma unroll
+                for (int i = 0; i < kRun; i++) sq = fmaf(v[k][i], v[k][i], sq);
+            }
+        }
+        const float rstd = 1.0f / sqrtf(sum(sq, 0.0f, step).x / (float)a.cols + a.eps);
+        if (a.rstd && lane == 0) a.rstd[row] = rstd;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const uint32_t col = (k * TPR + lane) * kRun;
+            if (col >= a.cols) continue;
+#pragma unroll
+            for (int i = 0; i < kRun; i++) v[k][i] *= rstd * w[k][i];
+            Run<DT> run;
+            run.set(v[k]);
+            T* out = static_cast<T*>(a.out) + row * a.out_stride + col;
+            if (col + kRun <= a.cols) run.store(out);
+            else run.store_part(out, (int)a.cols - (int)col);
+        }
+    }
+}
+
+// What a thread reads of one row.
+template <uint32_t DT, int NV>
+struct GradRow {
+    uint4 codes[NV];
+    uint32_t byte[NV];
+    Run<DT> dy[NV], dres[NV];
+
+    template <int TPR>
+    __device__ __forceinline__ void load(const NormArgs& a, uint32_t row) {
+        using T = typename Elem<DT>::T;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const uint32_t col = (k * TPR + threadIdx.x % TPR) * kRun;
+            const int n = (int)a.cols - (int)col;
+            if (n <= 0) continue;
+            const T* dy_at = static_cast<const T*>(a.dy) + row * a.dy_stride + col;
+            const T* dres_at = static_cast<const T*>(a.dres) + row * a.dres_stride + col;
+            codes[k] = load_codes(a.codes + row * a.code_stride + col, n);
+            byte[k] = a.scales[(uint64_t)row * a.blocks + col / kBlock];
+            if (n >= kRun) {
+                dy[k].load(dy_at);
+                if (a.dres) dres[k].load(dres_at);
+            } else {
+                dy[k].load_part(dy_at, n);
+                if (a.dres) dres[k].load_part(dres_at, n);
+            }
+        }
+    }
+};
+
+template <uint32_t DT, int TPR, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS, GRAD_CTAS)
+norm_grad_vec_kernel(NormArgs a) {
+    using T = typename Elem<DT>::T;
+    __shared__ RowSum<TPR, THREADS> sum;
+    const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows, at_once = THREADS / TPR;
+    float w[NV][kRun], dw[NV][kRun];
+    load_weights<TPR, NV>(a, w);
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int i = 0; i < kRun; i++) dw[k][i] = 0.0f;
+    uint32_t step = 0;
+    uint32_t row = blockIdx.x * at_once + threadIdx.x / TPR;
+    GradRow<DT, NV> next;
+    constexpr bool kAhead = DT != RLCU_F32;    // FP32 rows take twice the registers: two of them would spill
+    if (kAhead && row < rows) next.template load<TPR>(a, row);
+    // (all threads of a CTA take the same number of steps where a barrier is among them: TPR = THREADS)
+    for (; row < rows; row += gridDim.x * at_once, step++) {
+        if (!kAhead) next.template load<TPR>(a, row);
+        const GradRow<DT, NV> now = next;
+        if (kAhead && row + gridDim.x * at_once < rows) next.template load<TPR>(a, row + gridDim.x * at_once);
+        float sq = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            if ((k * TPR + lane) * kRun >= a.cols) continue;
+            float v[kRun], d[kRun];
+            decode_run(now.codes[k], now.byte[k], v);
+            now.dy[k].get(d);
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                sq = fmaf(v[i], v[i], sq);
+                dot = fmaf(d[i] * w[k][i], v[i], dot);
+            }
+        }
+        const float2 sums = sum(sq, dot, step);
+        const float rstd = 1.0f / sqrtf(sums.x / (float)a.cols + a.eps);
+        const float pull = sums.y / (float)a.cols * rstd * rstd;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const uint32_t col = (k * TPR + lane) * kRun;
+            if (col >= a.cols) continue;
+            float v[kRun], d[kRun], r[kRun];
+            decode_run(now.codes[k], now.byte[k], v);
+            now.dy[k].get(d);
+            if (a.dres) now.dres[k].get(r);
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                dw[k][i] = fmaf(d[i], v[i] * rstd, dw[k][i]);
+                const float g = fmaf(-v[i], pull, d[i] * w[k][i]);
+                d[i] = a.dres ? fmaf(rstd, g, r[i]) : rstd * g;
+            }
+            Run<DT> run;
+            run.set(d);
+            T* out = static_cast<T*>(a.out) + row * a.out_stride + col;
+            if (col + kRun <= a.cols) run.store(out);
+            else run.store_part(out, (int)a.cols - (int)col);
+        }
+    }
+    if (!a.partial) return;
+    float* part = a.partial + (uint64_t)blockIdx.x * a.cols;
+    if constexpr (TPR == 32) {
+        // the CTA's warps have the same columns: warp 0 to the last, in turn
+        __shared__ float shared[NV * 32 * kRun];
+        for (int turn = 0; turn < (int)at_once; turn++) {
+            if (threadIdx.x / TPR == turn)
+#pragma unroll
+                for (int k = 0; k < NV; k++)
+#pragma unroll
+                    for (int i = 0; i < kRun; i++) {
+                        float* s = shared + (k * kRun + i) * 32 + lane;
+                        *s = turn ? *s + dw[k][i] : dw[k][i];
+                    }
+            __syncthreads();
+        }
+        for (uint32_t j = threadIdx.x; j < a.cols; j += THREADS) {
+            const uint32_t run = j / kRun;
+            part[j] = shared[(run / 32 * kRun + j % kRun) * 32 + run % 32];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                const uint32_t j = (k * TPR + lane) * kRun + i;
+                if (j < a.cols) part[j] = dw[k][i];
+            }
+    }
+}
+
+// dweight from the CTAs' partial sums: a CTA per 32 columns, a warp per eighth of the parts, then the warps in order.
 __global__ void __launch_bounds__(kAct8Threads)
 norm_weight_kernel(const float* partial, uint32_t parts, uint32_t cols, float* dweight, uint32_t flags) {
-    for (uint32_t j = blockIdx.x * kAct8Threads + threadIdx.x; j < cols; j += gridDim.x * kAct8Threads) {
-        float s = 0.0f;
-        for (uint32_t p = 0; p < parts; p++) s += partial[(uint64_t)p * cols + j];
+    __shared__ float sums[kAct8Threads / 32][32];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
+    float s = 0.0f;
+    if (j < cols)
+#pragma unroll 8
+        for (uint32_t p = warp; p < parts; p += kAct8Threads / 32) s += partial[(uint64_t)p * cols + j];
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && j < cols) {
+        s = sums[0][lane];
+#pragma unroll
+        for (int w = 1; w < kAct8Threads / 32; w++) s += sums[w][lane];
         dweight[j] = flags & RLCU_ACT8_ACCUMULATE ? dweight[j] + s : s;
     }
 }
@@ -224,9 +648,11 @@ norm_weight_kernel(const float* partial, uint32_t parts, uint32_t cols, float* d
 // host side
 // ---------------------------------------------------------------------------
 
-constexpr uint64_t kMostParts = 296;      // rows are dealt to at most this many CTAs where dweight is asked for
-
-uint64_t norm_parts(uint64_t rows) { return rows < kMostParts ? rows : kMostParts; }
+// CTAs the rows of a gradient are dealt to, at most: eight, four or two per SM by the width that decides their threads
+uint64_t norm_parts(uint64_t rows, uint64_t cols) {
+    const uint64_t most = GRAD_PARTS * (cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1);
+    return rows < most ? rows : most;
+}
 
 int check_matrix(const char* what, const void* p, uint32_t dtype, uint64_t rows, uint64_t cols, uint64_t& stride) {
     if (!dtype_known(dtype)) return set_error(RLCU_ERR_INVALID, "unknown dtype %u", dtype);
@@ -251,12 +677,69 @@ bool same_or_apart(const void* p, uint64_t ps, const void* q, uint64_t qs, uint6
     return !overlap(span_of(p, rows, cols, ps, esz), span_of(q, rows, cols, qs, esz));
 }
 
+// every row starts on a 16-byte boundary
+bool rows16(const void* p, uint64_t stride, size_t esz, uint64_t rows) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || stride * esz % 16 == 0);
+}
+
 int grid_for(uint64_t units, int per_sm, int* out) {
     int dev = 0, sms = 0;
     RLCU_CUDA(cudaGetDevice(&dev));
     RLCU_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     const uint64_t most = (uint64_t)sms * per_sm;
     *out = (int)(units < most ? units : most);
+    return RLCU_OK;
+}
+
+constexpr uint64_t kMostVecCols = 8192;
+
+template <uint32_t DT, int TPR, int NV, int THREADS>
+int launch_norm_vec(const NormArgs& a, cudaStream_t s) {
+    // a few rows per CTA, so that their weights are read once for them; the grid moves through memory in order
+    uint32_t per = THREADS / TPR * 4;
+    while (per > THREADS / TPR && a.rows / per < 1184) per /= 2;
+    norm_vec_kernel<DT, TPR, NV, THREADS><<<(unsigned)((a.rows + per - 1) / per), THREADS, 0, s>>>(a, per);
+    RLCU_CUDA(cudaGetLastError());
+    return RLCU_OK;
+}
+
+template <uint32_t DT>
+int launch_norm(const NormArgs& a, bool vec, cudaStream_t s) {
+    if (vec) {
+        if (a.cols <= 512) return launch_norm_vec<DT, 32, 1, 256>(a, s);
+        if (a.cols <= 1024) return launch_norm_vec<DT, 32, 2, 256>(a, s);
+        if (a.cols <= 2048) return launch_norm_vec<DT, 128, 1, 128>(a, s);
+        if (a.cols <= 4096) return launch_norm_vec<DT, 256, 1, 256>(a, s);
+        return launch_norm_vec<DT, 512, 1, 512>(a, s);
+    }
+    int grid = 0;
+    if (const int rc = grid_for(a.rows, 8, &grid)) return rc;
+    norm_kernel<DT><<<grid, kAct8Threads, 0, s>>>(a);
+    RLCU_CUDA(cudaGetLastError());
+    return RLCU_OK;
+}
+
+template <uint32_t DT, int TPR, int NV, int THREADS>
+int launch_norm_grad_vec(const NormArgs& a, int* parts, cudaStream_t s) {
+    const uint64_t at_once = THREADS / TPR, steps = (a.rows + at_once - 1) / at_once;
+    *parts = (int)norm_parts(steps, a.cols);
+    norm_grad_vec_kernel<DT, TPR, NV, THREADS><<<*parts, THREADS, 0, s>>>(a);
+    RLCU_CUDA(cudaGetLastError());
+    return RLCU_OK;
+}
+
+template <uint32_t DT>
+int launch_norm_grad(const NormArgs& a, bool vec, int* parts, cudaStream_t s) {
+    if (vec) {
+        if (a.cols <= 512) return launch_norm_grad_vec<DT, 32, 1, 256>(a, parts, s);
+        if (a.cols <= 1024) return launch_norm_grad_vec<DT, 64, 1, 64>(a, parts, s);
+        if (a.cols <= 2048) return launch_norm_grad_vec<DT, 128, 1, 128>(a, parts, s);
+        if (a.cols <= 4096) return launch_norm_grad_vec<DT, 256, 1, 256>(a, parts, s);
+        return launch_norm_grad_vec<DT, 512, 1, 512>(a, parts, s);
+    }
+    *parts = (int)norm_parts(a.rows, a.cols);
+    norm_grad_kernel<DT><<<*parts, kAct8Threads, 0, s>>>(a);
+    RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
 }
 
@@ -267,7 +750,7 @@ using namespace rlcu;
 
 extern "C" uint64_t rlcu_act8_blocks(uint64_t cols) { return (cols + kBlock - 1) / kBlock; }
 
-extern "C" uint64_t rlcu_act8_rmsnorm_grad_workspace(uint64_t rows, uint64_t cols) { return norm_parts(rows) * cols * sizeof(float); }
+extern "C" uint64_t rlcu_act8_rmsnorm_grad_workspace(uint64_t rows, uint64_t cols) { return norm_parts(rows, cols) * cols * sizeof(float); }
 
 extern "C" int rlcu_act8_store(const void* x, uint32_t dtype, uint64_t rows, uint64_t cols, uint64_t x_stride,
                                uint8_t* codes, uint64_t code_stride, uint8_t* scales, void* stream) {
@@ -276,12 +759,22 @@ extern "C" int rlcu_act8_store(const void* x, uint32_t dtype, uint64_t rows, uin
     if (!rows || !cols) return RLCU_OK;
     if (overlap(span_of(x, rows, cols, x_stride, dtype_bytes(dtype)), span_of(codes, rows, cols, code_stride, 1)))
         return set_error(RLCU_ERR_INVALID, "x and codes overlap");
-    int grid = 0;
-    if (const int rc = grid_for((rows * rlcu_act8_blocks(cols) + 7) / 8, 8, &grid)) return rc;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == RLCU_F16) act8_store_kernel<RLCU_F16><<<grid, kAct8Threads, 0, s>>>(x, rows, (uint32_t)cols, x_stride, codes, code_stride, scales);
-    else if (dtype == RLCU_BF16) act8_store_kernel<RLCU_BF16><<<grid, kAct8Threads, 0, s>>>(x, rows, (uint32_t)cols, x_stride, codes, code_stride, scales);
-    else act8_store_kernel<RLCU_F32><<<grid, kAct8Threads, 0, s>>>(x, rows, (uint32_t)cols, x_stride, codes, code_stride, scales);
+    const uint64_t blocks = rlcu_act8_blocks(cols), total = rows * blocks;
+    if (rows16(x, x_stride, dtype_bytes(dtype), rows) && rows16(codes, code_stride, 1, rows) && total <= 0x7FFFFFFFull) {
+        const unsigned grid = (unsigned)((total + kVecBlocks - 1) / kVecBlocks);
+#define RLCU_STORE(DT) act8_store_vec_kernel<DT><<<grid, kAct8Threads, 0, s>>>(x, (uint32_t)total, (uint32_t)blocks, (uint32_t)cols, x_stride, codes, code_stride, scales)
+        if (dtype == RLCU_F16) RLCU_STORE(RLCU_F16);
+        else if (dtype == RLCU_BF16) RLCU_STORE(RLCU_BF16);
+        else RLCU_STORE(RLCU_F32);
+#undef RLCU_STORE
+    } else {
+        int grid = 0;
+        if (const int rc = grid_for((total + 7) / 8, 8, &grid)) return rc;
+        if (dtype == RLCU_F16) act8_store_kernel<RLCU_F16><<<grid, kAct8Threads, 0, s>>>(x, rows, (uint32_t)cols, x_stride, codes, code_stride, scales);
+        else if (dtype == RLCU_BF16) act8_store_kernel<RLCU_BF16><<<grid, kAct8Threads, 0, s>>>(x, rows, (uint32_t)cols, x_stride, codes, code_stride, scales);
+        else act8_store_kernel<RLCU_F32><<<grid, kAct8Threads, 0, s>>>(x, rows, (uint32_t)cols, x_stride, codes, code_stride, scales);
+    }
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
 }
@@ -293,12 +786,22 @@ extern "C" int rlcu_act8_load(const uint8_t* codes, uint64_t code_stride, const 
     if (!rows || !cols) return RLCU_OK;
     if (overlap(span_of(x, rows, cols, x_stride, dtype_bytes(dtype)), span_of(codes, rows, cols, code_stride, 1)))
         return set_error(RLCU_ERR_INVALID, "x and codes overlap");
-    int grid = 0;
-    if (const int rc = grid_for((rows * rlcu_act8_blocks(cols) + 7) / 8, 8, &grid)) return rc;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == RLCU_F16) act8_load_kernel<RLCU_F16><<<grid, kAct8Threads, 0, s>>>(codes, code_stride, scales, rows, (uint32_t)cols, x, x_stride);
-    else if (dtype == RLCU_BF16) act8_load_kernel<RLCU_BF16><<<grid, kAct8Threads, 0, s>>>(codes, code_stride, scales, rows, (uint32_t)cols, x, x_stride);
-    else act8_load_kernel<RLCU_F32><<<grid, kAct8Threads, 0, s>>>(codes, code_stride, scales, rows, (uint32_t)cols, x, x_stride);
+    const uint64_t blocks = rlcu_act8_blocks(cols), total = rows * blocks;
+    if (rows16(x, x_stride, dtype_bytes(dtype), rows) && rows16(codes, code_stride, 1, rows) && total <= 0x7FFFFFFFull) {
+        const unsigned grid = (unsigned)((total + kVecBlocks - 1) / kVecBlocks);
+#define RLCU_LOAD(DT) act8_load_vec_kernel<DT><<<grid, kAct8Threads, 0, s>>>(codes, code_stride, scales, (uint32_t)total, (uint32_t)blocks, (uint32_t)cols, x, x_stride)
+        if (dtype == RLCU_F16) RLCU_LOAD(RLCU_F16);
+        else if (dtype == RLCU_BF16) RLCU_LOAD(RLCU_BF16);
+        else RLCU_LOAD(RLCU_F32);
+#undef RLCU_LOAD
+    } else {
+        int grid = 0;
+        if (const int rc = grid_for((total + 7) / 8, 8, &grid)) return rc;
+        if (dtype == RLCU_F16) act8_load_kernel<RLCU_F16><<<grid, kAct8Threads, 0, s>>>(codes, code_stride, scales, rows, (uint32_t)cols, x, x_stride);
+        else if (dtype == RLCU_BF16) act8_load_kernel<RLCU_BF16><<<grid, kAct8Threads, 0, s>>>(codes, code_stride, scales, rows, (uint32_t)cols, x, x_stride);
+        else act8_load_kernel<RLCU_F32><<<grid, kAct8Threads, 0, s>>>(codes, code_stride, scales, rows, (uint32_t)cols, x, x_stride);
+    }
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
 }
@@ -316,14 +819,11 @@ extern "C" int rlcu_act8_rmsnorm(const uint8_t* codes, uint64_t code_stride, con
         return set_error(RLCU_ERR_INVALID, "y and codes overlap");
     NormArgs a = {codes, code_stride, scales, rows, (uint32_t)cols, (uint32_t)rlcu_act8_blocks(cols), weight, weight_dtype, eps,
                   nullptr, 0, nullptr, 0, y, y_stride, rstd, nullptr};
-    int grid = 0;
-    if (const int rc = grid_for(rows, 8, &grid)) return rc;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == RLCU_F16) norm_kernel<RLCU_F16><<<grid, kAct8Threads, 0, s>>>(a);
-    else if (dtype == RLCU_BF16) norm_kernel<RLCU_BF16><<<grid, kAct8Threads, 0, s>>>(a);
-    else norm_kernel<RLCU_F32><<<grid, kAct8Threads, 0, s>>>(a);
-    RLCU_CUDA(cudaGetLastError());
-    return RLCU_OK;
+    const bool vec = rows16(codes, code_stride, 1, rows) && rows16(y, y_stride, dtype_bytes(dtype), rows) && cols <= kMostVecCols;
+    if (dtype == RLCU_F16) return launch_norm<RLCU_F16>(a, vec, s);
+    if (dtype == RLCU_BF16) return launch_norm<RLCU_BF16>(a, vec, s);
+    return launch_norm<RLCU_F32>(a, vec, s);
 }
 
 extern "C" int rlcu_act8_rmsnorm_grad(const uint8_t* codes, uint64_t code_stride, const uint8_t* scales, uint64_t rows,
@@ -354,16 +854,17 @@ extern "C" int rlcu_act8_rmsnorm_grad(const uint8_t* codes, uint64_t code_stride
     NormArgs a = {codes, code_stride, scales, rows, (uint32_t)cols, (uint32_t)rlcu_act8_blocks(cols), weight, weight_dtype, eps,
                   dy, dy_stride, dresidual, dresidual_stride, dx, dx_stride, nullptr,
                   dweight ? static_cast<float*>(workspace) : nullptr};
-    const int grid = (int)norm_parts(rows);
-    if (grid) {
-        if (dtype == RLCU_F16) norm_grad_kernel<RLCU_F16><<<grid, kAct8Threads, 0, s>>>(a);
-        else if (dtype == RLCU_BF16) norm_grad_kernel<RLCU_BF16><<<grid, kAct8Threads, 0, s>>>(a);
-        else norm_grad_kernel<RLCU_F32><<<grid, kAct8Threads, 0, s>>>(a);
-        RLCU_CUDA(cudaGetLastError());
+    const bool vec = rows16(codes, code_stride, 1, rows) && rows16(dy, dy_stride, esz, rows) && rows16(dx, dx_stride, esz, rows) &&
+                     (!dresidual || rows16(dresidual, dresidual_stride, esz, rows)) && cols <= kMostVecCols;
+    int parts = 0;
+    if (rows) {
+        const int rc = dtype == RLCU_F16    ? launch_norm_grad<RLCU_F16>(a, vec, &parts, s)
+                       : dtype == RLCU_BF16 ? launch_norm_grad<RLCU_BF16>(a, vec, &parts, s)
+                                            : launch_norm_grad<RLCU_F32>(a, vec, &parts, s);
+        if (rc) return rc;
     }
     if (dweight) {
-        norm_weight_kernel<<<(int)((cols + kAct8Threads - 1) / kAct8Threads), kAct8Threads, 0, s>>>(a.partial, (uint32_t)grid,
-                                                                                                  (uint32_t)cols, dweight, flags);
+        norm_weight_kernel<<<(unsigned)((cols + 31) / 32), kAct8Threads, 0, s>>>(a.partial, (uint32_t)parts, (uint32_t)cols, dweight, flags);
         RLCU_CUDA(cudaGetLastError());
     }
     return RLCU_OK;
