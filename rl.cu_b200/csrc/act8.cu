@@ -456,15 +456,34 @@ struct RowSum {
     }
 };
 
+template <uint32_t DT>
+__device__ __forceinline__ void load_weight_run(const void* weight, uint32_t col, int n, float (&w)[kRun]) {
+    using E = Elem<DT>;
+    const typename E::T* p = static_cast<const typename E::T*>(weight) + col;
+    if (n >= kRun && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+#pragma unroll
+        for (int i = 0; i < kRun / E::kVec; i++) {
+            float g[E::kVec];
+            E::unpack(__ldg(reinterpret_cast<const uint4*>(p) + i), g);
+#pragma unroll
+            for (int q = 0; q < E::kVec; q++) w[i * E::kVec + q] = g[q];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRun; i++) w[i] = i < n ? E::up(p[i]) : 0.0f;
+    }
+}
+
 template <int TPR, int NV>
 __device__ __forceinline__ void load_weights(const NormArgs& a, float (&w)[NV][kRun]) {
 #pragma unroll
-    for (int k = 0; k < NV; k++)
-#pragma unroll
-        for (int i = 0; i < kRun; i++) {
-            const uint32_t j = (k * TPR + threadIdx.x % TPR) * kRun + i;
-            w[k][i] = j < a.cols ? weight_at(a, j) : 0.0f;
-        }
+    for (int k = 0; k < NV; k++) {
+        const uint32_t col = (k * TPR + threadIdx.x % TPR) * kRun;
+        const int n = (int)a.cols - (int)col;
+        if (a.weight_dtype == RLCU_F32) load_weight_run<RLCU_F32>(a.weight, col, n, w[k]);
+        else if (a.weight_dtype == RLCU_BF16) load_weight_run<RLCU_BF16>(a.weight, col, n, w[k]);
+        else load_weight_run<RLCU_F16>(a.weight, col, n, w[k]);
+    }
 }
 
 template <uint32_t DT, int TPR, int NV, int THREADS>
@@ -697,7 +716,7 @@ template <uint32_t DT, int TPR, int NV, int THREADS>
 int launch_norm_vec(const NormArgs& a, cudaStream_t s) {
     // a few rows per CTA, so that their weights are read once for them; the grid moves through memory in order
     uint32_t per = THREADS / TPR * 4;
-    while (per > THREADS / TPR && a.rows / per < 1184) per /= 2;
+    while (per > THREADS / TPR && a.rows / per < 148 * 2048 / THREADS) per /= 2;
     norm_vec_kernel<DT, TPR, NV, THREADS><<<(unsigned)((a.rows + per - 1) / per), THREADS, 0, s>>>(a, per);
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
@@ -707,7 +726,7 @@ template <uint32_t DT>
 int launch_norm(const NormArgs& a, bool vec, cudaStream_t s) {
     if (vec) {
         if (a.cols <= 512) return launch_norm_vec<DT, 32, 1, 256>(a, s);
-        if (a.cols <= 1024) return launch_norm_vec<DT, 32, 2, 256>(a, s);
+        if (a.cols <= 1024) return launch_norm_vec<DT, 64, 1, 64>(a, s);
         if (a.cols <= 2048) return launch_norm_vec<DT, 128, 1, 128>(a, s);
         if (a.cols <= 4096) return launch_norm_vec<DT, 256, 1, 256>(a, s);
         return launch_norm_vec<DT, 512, 1, 512>(a, s);
