@@ -186,6 +186,31 @@ struct Run {
         }
     }
 };
+constexpr int kPairs = kRun / 2;
+
+// 16 columns as pairs of FP32 (for the packed arithmetic)
+template <uint32_t DT>
+__device__ __forceinline__ void to_pairs(const Run<DT>& r, F2 (&p)[kPairs]) {
+    float f[kRun];
+    r.get(f);
+#pragma unroll
+    for (int i = 0; i < kPairs; i++) p[i] = F2(f[2 * i], f[2 * i + 1]);
+}
+template <uint32_t DT>
+__device__ __forceinline__ Run<DT> from_pairs(const F2 (&p)[kPairs]) {
+    float f[kRun];
+#pragma unroll
+    for (int i = 0; i < kPairs; i++) p[i].get(f[2 * i], f[2 * i + 1]);
+    Run<DT> r;
+    r.set(f);
+    return r;
+}
+__device__ __forceinline__ float add_pairs(F2 a) {
+    float x, y;
+    a.get(x, y);
+    return x + y;
+}
+
 // the codes of 16 columns, the first n of them where the row ends sooner
 __device__ __forceinline__ uint4 load_codes(const uint8_t* p, int n) {
     if (n >= kRun) return __ldcs(reinterpret_cast<const uint4*>(p));
@@ -211,6 +236,16 @@ __device__ __forceinline__ void decode4(uint32_t w, float* f) {
     f[1] = x.y;
     f[2] = y.x;
     f[3] = y.y;
+}
+// 16 codes without their scale
+__device__ __forceinline__ void code_pairs(uint4 v, F2 (&p)[kPairs]) {
+    float f[kRun];
+    decode4(v.x, f);
+    decode4(v.y, f + 4);
+    decode4(v.z, f + 8);
+    decode4(v.w, f + 12);
+#pragma unroll
+    for (int i = 0; i < kPairs; i++) p[i] = F2(f[2 * i], f[2 * i + 1]);
 }
 // 16 codes as values, before any rounding; finite ones stay finite
 __device__ __forceinline__ void decode_run(uint4 v, uint32_t byte, float (&f)[kRun]) {
@@ -430,9 +465,9 @@ norm_grad_kernel(NormArgs a) {
     }
 }
 
-// Rows that start on 16-byte boundaries: TPR threads per row, each with the same NV runs of 16 columns of every row it
-// works on (so their weights stay in registers), a CTA with THREADS / TPR rows at a time.  The row is decoded once; the
-// sums over it go through one barrier (none where a warp has the row).
+// Rows that start on 16-byte boundaries: TPR threads per row, each with the same run of 16 columns of every row it works
+// on (so their weights stay in registers), a CTA with THREADS / TPR rows at a time.  The row is decoded once; the sums
+// over it go through one barrier (none where a warp has the row).
 template <int TPR, int THREADS>
 struct RowSum {
     float2 part[2][THREADS / 32];              // by step parity
@@ -474,173 +509,221 @@ __device__ __forceinline__ void load_weight_run(const void* weight, uint32_t col
     }
 }
 
-template <int TPR, int NV>
-__device__ __forceinline__ void load_weights(const NormArgs& a, float (&w)[NV][kRun]) {
+__device__ __forceinline__ void load_weights(const NormArgs& a, uint32_t col, int n, F2 (&w)[kPairs]) {
+    float f[kRun];
+    if (a.weight_dtype == RLCU_F32) load_weight_run<RLCU_F32>(a.weight, col, n, f);
+    else if (a.weight_dtype == RLCU_BF16) load_weight_run<RLCU_BF16>(a.weight, col, n, f);
+    else load_weight_run<RLCU_F16>(a.weight, col, n, f);
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-        const uint32_t col = (k * TPR + threadIdx.x % TPR) * kRun;
-        const int n = (int)a.cols - (int)col;
-        if (a.weight_dtype == RLCU_F32) load_weight_run<RLCU_F32>(a.weight, col, n, w[k]);
-        else if (a.weight_dtype == RLCU_BF16) load_weight_run<RLCU_BF16>(a.weight, col, n, w[k]);
-        else load_weight_run<RLCU_F16>(a.weight, col, n, w[k]);
-    }
+    for (int i = 0; i < kPairs; i++) w[i] = F2(f[2 * i], f[2 * i + 1]);
 }
 
-template <uint32_t DT, int TPR, int NV, int THREADS>
+// A thread's 16 columns lie in one block, so their scale s comes out of the sums: sum x^2 = s^2 sum c^2 and so on, with
+// c the codes, and x itself is never formed.
+template <uint32_t DT, int TPR, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 norm_vec_kernel(NormArgs a, uint32_t rows_per_cta) {
     using T = typename Elem<DT>::T;
     __shared__ RowSum<TPR, THREADS> sum;
-    const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows;
+    const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows, col = lane * kRun;
+    const int n = (int)a.cols - (int)col;
     const uint32_t first = blockIdx.x * rows_per_cta + threadIdx.x / TPR, last = min(rows, (blockIdx.x + 1) * rows_per_cta);
-    float w[NV][kRun];
-    load_weights<TPR, NV>(a, w);
+    F2 w[kPairs];
+    load_weights(a, col, n, w);
+    uint4 codes;
+    uint32_t byte = 0;
+    auto fetch = [&](uint32_t row) {
+        if (row < last && n > 0) {
+            codes = load_codes(a.codes + row * a.code_stride + col, n);
+            byte = a.scales[(uint64_t)row * a.blocks + col / kBlock];
+        }
+    };
+    fetch(first);
     uint32_t step = 0;
     for (uint32_t row = first; row < last; row += THREADS / TPR, step++) {
-        float v[NV][kRun], sq = 0.0f;
+        F2 c[kPairs];
+        float sq = 0.0f;
+        const float s = pow2((int)byte - 127);
+        if (n > 0) {
+            code_pairs(codes, c);
+            F2 acc = mul2(c[0], c[0]);
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const uint32_t col = (k * TPR + lane) * kRun;
-            if (col < a.cols) {
-                decode_run(load_codes(a.codes + row * a.code_stride + col, (int)a.cols - (int)col), a.scales[(uint64_t)row * a.blocks + col / kBlock], v[k]);
-#pragma unroll
-                for (int i = 0; i < kRun; i++) sq = fmaf(v[k][i], v[k][i], sq);
-            }
+            for (int i = 1; i < kPairs; i++) acc = fma2(c[i], c[i], acc);
+            sq = s * (s * add_pairs(acc));
         }
+        fetch(row + THREADS / TPR);
         const float rstd = 1.0f / sqrtf(sum(sq, 0.0f, step).x / (float)a.cols + a.eps);
         if (a.rstd && lane == 0) a.rstd[row] = rstd;
+        if (n <= 0) continue;
+        const F2 k(s * rstd, s * rstd);
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const uint32_t col = (k * TPR + lane) * kRun;
-            if (col >= a.cols) continue;
-#pragma unroll
-            for (int i = 0; i < kRun; i++) v[k][i] *= rstd * w[k][i];
-            Run<DT> run;
-            run.set(v[k]);
-            T* out = static_cast<T*>(a.out) + row * a.out_stride + col;
-            if (col + kRun <= a.cols) run.store(out);
-            else run.store_part(out, (int)a.cols - (int)col);
-        }
+        for (int i = 0; i < kPairs; i++) c[i] = mul2(mul2(c[i], k), w[i]);
+        const Run<DT> run = from_pairs<DT>(c);
+        T* out = static_cast<T*>(a.out) + row * a.out_stride + col;
+        if (n >= kRun) run.store(out);
+        else run.store_part(out, n);
     }
 }
 
-// What a thread reads of one row.
-template <uint32_t DT, int NV>
-struct GradRow {
-    uint4 codes[NV];
-    uint32_t byte[NV];
-    Run<DT> dy[NV], dres[NV];
+// four columns of a run as two pairs, and back
+template <uint32_t DT>
+__device__ __forceinline__ void get_four(const Run<DT>& r, int i, F2 (&p)[2]) {
+    if constexpr (DT == RLCU_F32) {
+        const uint4 v = r.v[i];
+        p[0] = F2(__uint_as_float(v.x), __uint_as_float(v.y));
+        p[1] = F2(__uint_as_float(v.z), __uint_as_float(v.w));
+    } else {
+        const uint4 v = r.v[i / 2];
+        float a, b, c, d;
+        Elem<DT>::up2(i % 2 ? v.z : v.x, a, b);
+        Elem<DT>::up2(i % 2 ? v.w : v.y, c, d);
+        p[0] = F2(a, b);
+        p[1] = F2(c, d);
+    }
+}
+template <uint32_t DT>
+__device__ __forceinline__ void set_four(Run<DT>& r, int i, const F2 (&p)[2]) {
+    float a, b, c, d;
+    p[0].get(a, b);
+    p[1].get(c, d);
+    if constexpr (DT == RLCU_F32) {
+        r.v[i] = make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+    } else {
+        uint4& v = r.v[i / 2];
+        (i % 2 ? v.z : v.x) = Elem<DT>::down2(a, b);
+        (i % 2 ? v.w : v.y) = Elem<DT>::down2(c, d);
+    }
+}
 
-    template <int TPR>
-    __device__ __forceinline__ void load(const NormArgs& a, uint32_t row) {
-        using T = typename Elem<DT>::T;
+// What a thread reads of one row.  It stays packed between its two uses: unpacked it would not fit the registers.
+template <uint32_t DT>
+struct GradRow {
+    uint4 codes;
+    uint32_t byte;
+    Run<DT> dy, dres;
+
+    __device__ __forceinline__ void four(int i, F2 (&c)[2], F2 (&d)[2]) const {
+        float f[4];
+        decode4(i == 0 ? codes.x : i == 1 ? codes.y : i == 2 ? codes.z : codes.w, f);
+        c[0] = F2(f[0], f[1]);
+        c[1] = F2(f[2], f[3]);
+        get_four(dy, i, d);
+    }
+    __device__ __forceinline__ void four_dres(int i, F2 (&r)[2]) const { get_four(dres, i, r); }
+    __device__ __forceinline__ void keep_packed() {
+        asm volatile("" : "+r"(codes.x), "+r"(codes.y), "+r"(codes.z), "+r"(codes.w));
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const uint32_t col = (k * TPR + threadIdx.x % TPR) * kRun;
-            const int n = (int)a.cols - (int)col;
-            if (n <= 0) continue;
-            const T* dy_at = static_cast<const T*>(a.dy) + row * a.dy_stride + col;
-            const T* dres_at = static_cast<const T*>(a.dres) + row * a.dres_stride + col;
-            codes[k] = load_codes(a.codes + row * a.code_stride + col, n);
-            byte[k] = a.scales[(uint64_t)row * a.blocks + col / kBlock];
-            if (n >= kRun) {
-                dy[k].load(dy_at);
-                if (a.dres) dres[k].load(dres_at);
-            } else {
-                dy[k].load_part(dy_at, n);
-                if (a.dres) dres[k].load_part(dres_at, n);
-            }
-        }
+        for (int i = 0; i < Run<DT>::kGroups; i++)
+            asm volatile("" : "+r"(dy.v[i].x), "+r"(dy.v[i].y), "+r"(dy.v[i].z), "+r"(dy.v[i].w));
     }
 };
 
-template <uint32_t DT, int TPR, int NV, int THREADS>
+template <uint32_t DT, int TPR, int THREADS>
 __global__ void __launch_bounds__(THREADS, GRAD_CTAS)
 norm_grad_vec_kernel(NormArgs a) {
     using T = typename Elem<DT>::T;
-    __shared__ RowSum<TPR, THREADS> sum;
-    const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows, at_once = THREADS / TPR;
-    float w[NV][kRun], dw[NV][kRun];
-    load_weights<TPR, NV>(a, w);
-#pragma unroll
-    for (int k = 0; k < NV; k++)
-#pragma unroll
-        for (int i = 0; i < kRun; i++) dw[k][i] = 0.0f;
-    uint32_t step = 0;
-    uint32_t row = blockIdx.x * at_once + threadIdx.x / TPR;
-    GradRow<DT, NV> next;
     constexpr bool kAhead = DT != RLCU_F32;    // FP32 rows take twice the registers: two of them would spill
-    if (kAhead && row < rows) next.template load<TPR>(a, row);
-    // (all threads of a CTA take the same number of steps where a barrier is among them: TPR = THREADS)
-    for (; row < rows; row += gridDim.x * at_once, step++) {
-        if (!kAhead) next.template load<TPR>(a, row);
-        const GradRow<DT, NV> now = next;
-        if (kAhead && row + gridDim.x * at_once < rows) next.template load<TPR>(a, row + gridDim.x * at_once);
-        float sq = 0.0f, dot = 0.0f;
+    __shared__ RowSum<TPR, THREADS> sum;
+    const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows, at_once = THREADS / TPR, jump = gridDim.x * at_once;
+    const uint32_t col = lane * kRun;
+    const int n = (int)a.cols - (int)col;
+    F2 w[kPairs], dw[kPairs];
+    load_weights(a, col, n, w);
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            if ((k * TPR + lane) * kRun >= a.cols) continue;
-            float v[kRun], d[kRun];
-            decode_run(now.codes[k], now.byte[k], v);
-            now.dy[k].get(d);
-#pragma unroll
-            for (int i = 0; i < kRun; i++) {
-                sq = fmaf(v[i], v[i], sq);
-                dot = fmaf(d[i] * w[k][i], v[i], dot);
-            }
+    for (int i = 0; i < kPairs; i++) dw[i] = F2(0.0f, 0.0f);
+    uint32_t row = blockIdx.x * at_once + threadIdx.x / TPR;
+    const uint8_t* codes_at = a.codes + row * a.code_stride + col;
+    const uint8_t* scale_at = a.scales + (uint64_t)row * a.blocks + col / kBlock;
+    const T* dy_at = static_cast<const T*>(a.dy) + row * a.dy_stride + col;
+    const T* dres_at = static_cast<const T*>(a.dres) + row * a.dres_stride + col;
+    T* out = static_cast<T*>(a.out) + row * a.out_stride + col;
+    GradRow<DT> next;
+    auto fetch = [&]() {
+        if (n >= kRun) {
+            next.codes = __ldcs(reinterpret_cast<const uint4*>(codes_at));
+            next.dy.load(dy_at);
+            if (a.dres) next.dres.load(dres_at);
+        } else if (n > 0) {
+            next.codes = load_codes(codes_at, n);
+            next.dy.load_part(dy_at, n);
+            if (a.dres) next.dres.load_part(dres_at, n);
         }
+        next.byte = n > 0 ? *scale_at : 0u;
+        codes_at += (uint64_t)jump * a.code_stride;
+        scale_at += (uint64_t)jump * a.blocks;
+        dy_at += (uint64_t)jump * a.dy_stride;
+        dres_at += (uint64_t)jump * a.dres_stride;
+    };
+    if (kAhead && row < rows) fetch();
+    // (all threads of a CTA take the same number of steps where a barrier is among them: TPR = THREADS)
+    for (uint32_t step = 0; row < rows; row += jump, step++) {
+        if (!kAhead) fetch();
+        GradRow<DT> now = next;
+        const float s = pow2((int)now.byte - 127);
+        float sq = 0.0f, dot = 0.0f;
+        if (n > 0) {
+            F2 acc(0.0f, 0.0f), acc2(0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < kPairs; i += 2) {
+                F2 c[2], d[2];
+                now.four(i / 2, c, d);
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    acc = fma2(c[q], c[q], acc);
+                    acc2 = fma2(mul2(d[q], w[i + q]), c[q], acc2);
+                }
+            }
+            sq = s * (s * add_pairs(acc));
+            dot = s * add_pairs(acc2);
+        }
+        if (kAhead && row + jump < rows) fetch();
         const float2 sums = sum(sq, dot, step);
         const float rstd = 1.0f / sqrtf(sums.x / (float)a.cols + a.eps);
         const float pull = sums.y / (float)a.cols * rstd * rstd;
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const uint32_t col = (k * TPR + lane) * kRun;
-            if (col >= a.cols) continue;
-            float v[kRun], d[kRun], r[kRun];
-            decode_run(now.codes[k], now.byte[k], v);
-            now.dy[k].get(d);
-            if (a.dres) now.dres[k].get(r);
-#pragma unroll
-            for (int i = 0; i < kRun; i++) {
-                dw[k][i] = fmaf(d[i], v[i] * rstd, dw[k][i]);
-                const float g = fmaf(-v[i], pull, d[i] * w[k][i]);
-                d[i] = a.dres ? fmaf(rstd, g, r[i]) : rstd * g;
-            }
+        if (n > 0) {
+            const F2 to_dw(s * rstd, s * rstd), from_x(-(s * pull) * rstd, -(s * pull) * rstd), from_dy(rstd, rstd);
+            now.keep_packed();
             Run<DT> run;
-            run.set(d);
-            T* out = static_cast<T*>(a.out) + row * a.out_stride + col;
-            if (col + kRun <= a.cols) run.store(out);
-            else run.store_part(out, (int)a.cols - (int)col);
+#pragma unroll
+            for (int i = 0; i < kPairs; i += 2) {
+                F2 c[2], d[2], r[2];
+                now.four(i / 2, c, d);
+                if (a.dres) now.four_dres(i / 2, r);
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    dw[i + q] = fma2(d[q], mul2(c[q], to_dw), dw[i + q]);
+                    const F2 g = fma2(mul2(d[q], w[i + q]), from_dy, mul2(c[q], from_x));
+                    r[q] = a.dres ? add2(g, r[q]) : g;
+                }
+                set_four(run, i / 2, r);
+            }
+            if (n >= kRun) run.store(out);
+            else run.store_part(out, n);
         }
+        out += (uint64_t)jump * a.out_stride;
     }
     if (!a.partial) return;
     float* part = a.partial + (uint64_t)blockIdx.x * a.cols;
+    float f[kRun];
+#pragma unroll
+    for (int i = 0; i < kPairs; i++) dw[i].get(f[2 * i], f[2 * i + 1]);
     if constexpr (TPR == 32) {
         // the CTA's warps have the same columns: warp 0 to the last, in turn
-        __shared__ float shared[NV * 32 * kRun];
+        __shared__ float shared[32 * kRun];
         for (int turn = 0; turn < (int)at_once; turn++) {
             if (threadIdx.x / TPR == turn)
 #pragma unroll
-                for (int k = 0; k < NV; k++)
-#pragma unroll
-                    for (int i = 0; i < kRun; i++) {
-                        float* s = shared + (k * kRun + i) * 32 + lane;
-                        *s = turn ? *s + dw[k][i] : dw[k][i];
-                    }
+                for (int i = 0; i < kRun; i++) shared[i * 32 + lane] = turn ? shared[i * 32 + lane] + f[i] : f[i];
             __syncthreads();
         }
-        for (uint32_t j = threadIdx.x; j < a.cols; j += THREADS) {
-            const uint32_t run = j / kRun;
-            part[j] = shared[(run / 32 * kRun + j % kRun) * 32 + run % 32];
-        }
+        for (uint32_t j = threadIdx.x; j < a.cols; j += THREADS) part[j] = shared[j % kRun * 32 + j / kRun];
+    } else if (n >= kRun && a.cols % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < kRun; i += 4) *reinterpret_cast<float4*>(part + col + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
     } else {
 #pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int i = 0; i < kRun; i++) {
-                const uint32_t j = (k * TPR + lane) * kRun + i;
-                if (j < a.cols) part[j] = dw[k][i];
-            }
+        for (int i = 0; i < kRun; i++)
+            if (i < n) part[col + i] = f[i];
     }
 }
 
@@ -712,12 +795,12 @@ int grid_for(uint64_t units, int per_sm, int* out) {
 
 constexpr uint64_t kMostVecCols = 8192;
 
-template <uint32_t DT, int TPR, int NV, int THREADS>
+template <uint32_t DT, int TPR, int THREADS>
 int launch_norm_vec(const NormArgs& a, cudaStream_t s) {
     // a few rows per CTA, so that their weights are read once for them; the grid moves through memory in order
     uint32_t per = THREADS / TPR * 4;
     while (per > THREADS / TPR && a.rows / per < 148 * 2048 / THREADS) per /= 2;
-    norm_vec_kernel<DT, TPR, NV, THREADS><<<(unsigned)((a.rows + per - 1) / per), THREADS, 0, s>>>(a, per);
+    norm_vec_kernel<DT, TPR, THREADS><<<(unsigned)((a.rows + per - 1) / per), THREADS, 0, s>>>(a, per);
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
 }
@@ -725,11 +808,11 @@ int launch_norm_vec(const NormArgs& a, cudaStream_t s) {
 template <uint32_t DT>
 int launch_norm(const NormArgs& a, bool vec, cudaStream_t s) {
     if (vec) {
-        if (a.cols <= 512) return launch_norm_vec<DT, 32, 1, 256>(a, s);
-        if (a.cols <= 1024) return launch_norm_vec<DT, 64, 1, 64>(a, s);
-        if (a.cols <= 2048) return launch_norm_vec<DT, 128, 1, 128>(a, s);
-        if (a.cols <= 4096) return launch_norm_vec<DT, 256, 1, 256>(a, s);
-        return launch_norm_vec<DT, 512, 1, 512>(a, s);
+        if (a.cols <= 512) return launch_norm_vec<DT, 32, 256>(a, s);
+        if (a.cols <= 1024) return launch_norm_vec<DT, 64, 64>(a, s);
+        if (a.cols <= 2048) return launch_norm_vec<DT, 128, 128>(a, s);
+        if (a.cols <= 4096) return launch_norm_vec<DT, 256, 256>(a, s);
+        return launch_norm_vec<DT, 512, 512>(a, s);
     }
     int grid = 0;
     if (const int rc = grid_for(a.rows, 8, &grid)) return rc;
@@ -738,11 +821,11 @@ int launch_norm(const NormArgs& a, bool vec, cudaStream_t s) {
     return RLCU_OK;
 }
 
-template <uint32_t DT, int TPR, int NV, int THREADS>
+template <uint32_t DT, int TPR, int THREADS>
 int launch_norm_grad_vec(const NormArgs& a, int* parts, cudaStream_t s) {
     const uint64_t at_once = THREADS / TPR, steps = (a.rows + at_once - 1) / at_once;
     *parts = (int)norm_parts(steps, a.cols);
-    norm_grad_vec_kernel<DT, TPR, NV, THREADS><<<*parts, THREADS, 0, s>>>(a);
+    norm_grad_vec_kernel<DT, TPR, THREADS><<<*parts, THREADS, 0, s>>>(a);
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
 }
@@ -750,11 +833,11 @@ int launch_norm_grad_vec(const NormArgs& a, int* parts, cudaStream_t s) {
 template <uint32_t DT>
 int launch_norm_grad(const NormArgs& a, bool vec, int* parts, cudaStream_t s) {
     if (vec) {
-        if (a.cols <= 512) return launch_norm_grad_vec<DT, 32, 1, 256>(a, parts, s);
-        if (a.cols <= 1024) return launch_norm_grad_vec<DT, 64, 1, 64>(a, parts, s);
-        if (a.cols <= 2048) return launch_norm_grad_vec<DT, 128, 1, 128>(a, parts, s);
-        if (a.cols <= 4096) return launch_norm_grad_vec<DT, 256, 1, 256>(a, parts, s);
-        return launch_norm_grad_vec<DT, 512, 1, 512>(a, parts, s);
+        if (a.cols <= 512) return launch_norm_grad_vec<DT, 32, 256>(a, parts, s);
+        if (a.cols <= 1024) return launch_norm_grad_vec<DT, 64, 64>(a, parts, s);
+        if (a.cols <= 2048) return launch_norm_grad_vec<DT, 128, 128>(a, parts, s);
+        if (a.cols <= 4096) return launch_norm_grad_vec<DT, 256, 256>(a, parts, s);
+        return launch_norm_grad_vec<DT, 512, 512>(a, parts, s);
     }
     *parts = (int)norm_parts(a.rows, a.cols);
     norm_grad_kernel<DT><<<*parts, kAct8Threads, 0, s>>>(a);
