@@ -15,6 +15,9 @@
 #ifndef GRAD_CTAS
 #define GRAD_CTAS (512 / THREADS)
 #endif
+#ifndef FWD_ROWS
+#define FWD_ROWS 8
+#endif
 #ifndef GRAD_PARTS
 #define GRAD_PARTS 296
 #endif
@@ -471,21 +474,24 @@ norm_grad_kernel(NormArgs a) {
 template <int TPR, int THREADS>
 struct RowSum {
     float2 part[2][THREADS / 32];              // by step parity
+    // of the TPR threads that have the row
     __device__ __forceinline__ float2 operator()(float x, float y, uint32_t step) {
 #pragma unroll
         for (int mask = 16; mask >= 1; mask >>= 1) {
             x += __shfl_xor_sync(0xFFFFFFFFu, x, mask);
             y += __shfl_xor_sync(0xFFFFFFFFu, y, mask);
         }
-        if (TPR == 32) return make_float2(x, y);
-        static_assert(TPR == 32 || TPR == THREADS, "a warp or a CTA per row");
-        if ((threadIdx.x & 31) == 0) part[step & 1][threadIdx.x >> 5] = make_float2(x, y);
-        __syncthreads();
-        x = y = 0.0f;
+        if constexpr (TPR > 32) {
+            const uint32_t warp = threadIdx.x >> 5, group = threadIdx.x / TPR;
+            if ((threadIdx.x & 31) == 0) part[step & 1][warp] = make_float2(x, y);
+            if constexpr (TPR == THREADS) __syncthreads();
+            else asm volatile("barrier.cta.sync %0, %1;" :: "r"(group + 1), "n"(TPR) : "memory");
+            x = y = 0.0f;
 #pragma unroll
-        for (int w = 0; w < THREADS / 32; w++) {
-            x += part[step & 1][w].x;
-            y += part[step & 1][w].y;
+            for (int w = 0; w < TPR / 32; w++) {
+                x += part[step & 1][group * (TPR / 32) + w].x;
+                y += part[step & 1][group * (TPR / 32) + w].y;
+            }
         }
         return make_float2(x, y);
     }
@@ -530,38 +536,61 @@ norm_vec_kernel(NormArgs a, uint32_t rows_per_cta) {
     const uint32_t first = blockIdx.x * rows_per_cta + threadIdx.x / TPR, last = min(rows, (blockIdx.x + 1) * rows_per_cta);
     F2 w[kPairs];
     load_weights(a, col, n, w);
-    uint4 codes;
-    uint32_t byte = 0;
+    struct Held {
+        uint4 codes;
+        uint32_t byte;
+    } next[2];
+    constexpr uint32_t at_once = THREADS / TPR;
+    // two rows per step: one barrier for both
     auto fetch = [&](uint32_t row) {
-        if (row < last && n > 0) {
-            codes = load_codes(a.codes + row * a.code_stride + col, n);
-            byte = a.scales[(uint64_t)row * a.blocks + col / kBlock];
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const uint32_t at = row + r * at_once;
+            next[r].byte = 0;
+            next[r].codes = make_uint4(0u, 0u, 0u, 0u);
+            if (at < last && n > 0) {
+                next[r].codes = load_codes(a.codes + at * a.code_stride + col, n);
+                next[r].byte = a.scales[(uint64_t)at * a.blocks + col / kBlock];
+            }
         }
     };
     fetch(first);
     uint32_t step = 0;
-    for (uint32_t row = first; row < last; row += THREADS / TPR, step++) {
-        F2 c[kPairs];
-        float sq = 0.0f;
-        const float s = pow2((int)byte - 127);
-        if (n > 0) {
-            code_pairs(codes, c);
+    for (uint32_t row = first; row < last; row += 2 * at_once, step++) {
+        Held now[2] = {next[0], next[1]};
+        float sq[2];
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const float s = pow2((int)now[r].byte - 127);
+            F2 c[kPairs];
+            code_pairs(now[r].codes, c);
             F2 acc = mul2(c[0], c[0]);
 #pragma unroll
             for (int i = 1; i < kPairs; i++) acc = fma2(c[i], c[i], acc);
-            sq = s * (s * add_pairs(acc));
+            sq[r] = n > 0 ? s * (s * add_pairs(acc)) : 0.0f;
         }
-        fetch(row + THREADS / TPR);
-        const float rstd = 1.0f / sqrtf(sum(sq, 0.0f, step).x / (float)a.cols + a.eps);
-        if (a.rstd && lane == 0) a.rstd[row] = rstd;
-        if (n <= 0) continue;
-        const F2 k(s * rstd, s * rstd);
+        fetch(row + 2 * at_once);
+        const float2 sums = sum(sq[0], sq[1], step);
 #pragma unroll
-        for (int i = 0; i < kPairs; i++) c[i] = mul2(mul2(c[i], k), w[i]);
-        const Run<DT> run = from_pairs<DT>(c);
-        T* out = static_cast<T*>(a.out) + row * a.out_stride + col;
-        if (n >= kRun) run.store(out);
-        else run.store_part(out, n);
+        for (int r = 0; r < 2; r++) {
+            const uint32_t at = row + r * at_once;
+            if (at >= last) continue;
+            const float rstd = 1.0f / sqrtf((r ? sums.y : sums.x) / (float)a.cols + a.eps);
+            if (a.rstd && lane == 0) a.rstd[at] = rstd;
+            if (n <= 0) continue;
+            const float s = pow2((int)now[r].byte - 127) * rstd;
+            const F2 k(s, s);
+            // decoded again: packed, two rows fit the registers
+            asm volatile("" : "+r"(now[r].codes.x), "+r"(now[r].codes.y), "+r"(now[r].codes.z), "+r"(now[r].codes.w));
+            F2 c[kPairs];
+            code_pairs(now[r].codes, c);
+#pragma unroll
+            for (int i = 0; i < kPairs; i++) c[i] = mul2(mul2(c[i], k), w[i]);
+            const Run<DT> run = from_pairs<DT>(c);
+            T* out = static_cast<T*>(a.out) + at * a.out_stride + col;
+            if (n >= kRun) run.store(out);
+            else run.store_part(out, n);
+        }
     }
 }
 
@@ -655,7 +684,7 @@ norm_grad_vec_kernel(NormArgs a) {
         dres_at += (uint64_t)jump * a.dres_stride;
     };
     if (kAhead && row < rows) fetch();
-    // (all threads of a CTA take the same number of steps where a barrier is among them: TPR = THREADS)
+    // (the TPR threads that share a barrier take the same number of steps)
     for (uint32_t step = 0; row < rows; row += jump, step++) {
         if (!kAhead) fetch();
         GradRow<DT> now = next;
@@ -707,16 +736,16 @@ norm_grad_vec_kernel(NormArgs a) {
     float f[kRun];
 #pragma unroll
     for (int i = 0; i < kPairs; i++) dw[i].get(f[2 * i], f[2 * i + 1]);
-    if constexpr (TPR == 32) {
-        // the CTA's warps have the same columns: warp 0 to the last, in turn
-        __shared__ float shared[32 * kRun];
+    if constexpr (TPR < THREADS) {
+        // the CTA's groups have the same columns: the first to the last, in turn
+        __shared__ float shared[TPR * kRun];
         for (int turn = 0; turn < (int)at_once; turn++) {
             if (threadIdx.x / TPR == turn)
 #pragma unroll
-                for (int i = 0; i < kRun; i++) shared[i * 32 + lane] = turn ? shared[i * 32 + lane] + f[i] : f[i];
+                for (int i = 0; i < kRun; i++) shared[i * TPR + lane] = turn ? shared[i * TPR + lane] + f[i] : f[i];
             __syncthreads();
         }
-        for (uint32_t j = threadIdx.x; j < a.cols; j += THREADS) part[j] = shared[j % kRun * 32 + j / kRun];
+        for (uint32_t j = threadIdx.x; j < a.cols; j += THREADS) part[j] = shared[j % kRun * TPR + j / kRun];
     } else if (n >= kRun && a.cols % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < kRun; i += 4) *reinterpret_cast<float4*>(part + col + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
@@ -727,34 +756,37 @@ norm_grad_vec_kernel(NormArgs a) {
     }
 }
 
-// dweight from the CTAs' partial sums: a CTA per 32 columns, a warp per eighth of the parts, then the warps in order.
-__global__ void __launch_bounds__(kAct8Threads)
+// dweight from the CTAs' partial sums: a CTA per 32 columns, each warp every 32nd part, then the warps in order.  Launched
+// while the gradient kernel still runs; it waits for its end.
+constexpr int kWeightThreads = 1024;
+
+__global__ void __launch_bounds__(kWeightThreads)
 norm_weight_kernel(const float* partial, uint32_t parts, uint32_t cols, float* dweight, uint32_t flags) {
-    __shared__ float sums[kAct8Threads / 32][32];
+    __shared__ float sums[kWeightThreads / 32][33];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     float s = 0.0f;
     if (j < cols)
 #pragma unroll 8
-        for (uint32_t p = warp; p < parts; p += kAct8Threads / 32) s += partial[(uint64_t)p * cols + j];
+        for (uint32_t p = warp; p < parts; p += kWeightThreads / 32) s += partial[(uint64_t)p * cols + j];
     sums[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && j < cols) {
-        s = sums[0][lane];
+    // warp w: columns w of the 32, a lane per warp that summed
+    s = sums[lane][warp];
 #pragma unroll
-        for (int w = 1; w < kAct8Threads / 32; w++) s += sums[w][lane];
-        dweight[j] = flags & RLCU_ACT8_ACCUMULATE ? dweight[j] + s : s;
-    }
+    for (int mask = 16; mask >= 1; mask >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, mask);
+    const uint32_t out = blockIdx.x * 32 + warp;
+    if (lane == 0 && out < cols) dweight[out] = flags & RLCU_ACT8_ACCUMULATE ? dweight[out] + s : s;
 }
 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 
-// CTAs the rows of a gradient are dealt to, at most: eight, four or two per SM by the width that decides their threads
-uint64_t norm_parts(uint64_t rows, uint64_t cols) {
-    const uint64_t most = GRAD_PARTS * (cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1);
-    return rows < most ? rows : most;
-}
+// CTAs the rows of a gradient are dealt to, at most: what the registers of 148 SMs hold of 256 threads each
+constexpr uint64_t kMostParts = GRAD_PARTS;
+
+uint64_t norm_parts(uint64_t rows) { return rows < kMostParts ? rows : kMostParts; }
 
 int check_matrix(const char* what, const void* p, uint32_t dtype, uint64_t rows, uint64_t cols, uint64_t& stride) {
     if (!dtype_known(dtype)) return set_error(RLCU_ERR_INVALID, "unknown dtype %u", dtype);
@@ -798,8 +830,8 @@ constexpr uint64_t kMostVecCols = 8192;
 template <uint32_t DT, int TPR, int THREADS>
 int launch_norm_vec(const NormArgs& a, cudaStream_t s) {
     // a few rows per CTA, so that their weights are read once for them; the grid moves through memory in order
-    uint32_t per = THREADS / TPR * 4;
-    while (per > THREADS / TPR && a.rows / per < 148 * 2048 / THREADS) per /= 2;
+    uint32_t per = THREADS / TPR * FWD_ROWS;
+    while (per > THREADS / TPR * 2 && a.rows / per < 148 * 2048 / THREADS) per /= 2;
     norm_vec_kernel<DT, TPR, THREADS><<<(unsigned)((a.rows + per - 1) / per), THREADS, 0, s>>>(a, per);
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
@@ -824,7 +856,7 @@ int launch_norm(const NormArgs& a, bool vec, cudaStream_t s) {
 template <uint32_t DT, int TPR, int THREADS>
 int launch_norm_grad_vec(const NormArgs& a, int* parts, cudaStream_t s) {
     const uint64_t at_once = THREADS / TPR, steps = (a.rows + at_once - 1) / at_once;
-    *parts = (int)norm_parts(steps, a.cols);
+    *parts = (int)norm_parts(steps);
     norm_grad_vec_kernel<DT, TPR, THREADS><<<*parts, THREADS, 0, s>>>(a);
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
@@ -834,12 +866,12 @@ template <uint32_t DT>
 int launch_norm_grad(const NormArgs& a, bool vec, int* parts, cudaStream_t s) {
     if (vec) {
         if (a.cols <= 512) return launch_norm_grad_vec<DT, 32, 256>(a, parts, s);
-        if (a.cols <= 1024) return launch_norm_grad_vec<DT, 64, 64>(a, parts, s);
-        if (a.cols <= 2048) return launch_norm_grad_vec<DT, 128, 128>(a, parts, s);
+        if (a.cols <= 1024) return launch_norm_grad_vec<DT, 64, 256>(a, parts, s);
+        if (a.cols <= 2048) return launch_norm_grad_vec<DT, 128, 256>(a, parts, s);
         if (a.cols <= 4096) return launch_norm_grad_vec<DT, 256, 256>(a, parts, s);
         return launch_norm_grad_vec<DT, 512, 512>(a, parts, s);
     }
-    *parts = (int)norm_parts(a.rows, a.cols);
+    *parts = (int)norm_parts(a.rows);
     norm_grad_kernel<DT><<<*parts, kAct8Threads, 0, s>>>(a);
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
@@ -852,7 +884,7 @@ using namespace rlcu;
 
 extern "C" uint64_t rlcu_act8_blocks(uint64_t cols) { return (cols + kBlock - 1) / kBlock; }
 
-extern "C" uint64_t rlcu_act8_rmsnorm_grad_workspace(uint64_t rows, uint64_t cols) { return norm_parts(rows, cols) * cols * sizeof(float); }
+extern "C" uint64_t rlcu_act8_rmsnorm_grad_workspace(uint64_t rows, uint64_t cols) { return norm_parts(rows) * cols * sizeof(float); }
 
 extern "C" int rlcu_act8_store(const void* x, uint32_t dtype, uint64_t rows, uint64_t cols, uint64_t x_stride,
                                uint8_t* codes, uint64_t code_stride, uint8_t* scales, void* stream) {
@@ -966,8 +998,16 @@ extern "C" int rlcu_act8_rmsnorm_grad(const uint8_t* codes, uint64_t code_stride
         if (rc) return rc;
     }
     if (dweight) {
-        norm_weight_kernel<<<(unsigned)((cols + 31) / 32), kAct8Threads, 0, s>>>(a.partial, (uint32_t)parts, (uint32_t)cols, dweight, flags);
-        RLCU_CUDA(cudaGetLastError());
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)((cols + 31) / 32));
+        cfg.blockDim = dim3(kWeightThreads);
+        cfg.stream = s;
+        cfg.attrs = attr;
+        cfg.numAttrs = parts ? 1 : 0;
+        RLCU_CUDA(cudaLaunchKernelEx(&cfg, norm_weight_kernel, (const float*)a.partial, (uint32_t)parts, (uint32_t)cols, dweight, flags));
     }
     return RLCU_OK;
 }
