@@ -10,10 +10,10 @@
  *
  * Format: `rows` x `cols` values.  Each run of RLCU_ACT8_BLOCK consecutive columns of a row (the last one may be
  * shorter) has one byte s of scale, 2^e with e = s - 127, and one e4m3 code per value: value = code * 2^e.
- * e is the smallest exponent with max|x| <= 448 * 2^e, so a code is x * 2^-e rounded to nearest even
- * (relative error at most 2^-4 down to 2^-14 of a block's largest value, an absolute error of at most 2^-10 * 2^e below) and the
- * product with the scale is exact.  inf and NaN are kept as NaN; they do not enter max|x|.  A block of zeros has
- * s = 0.
+ * e is the smallest exponent (of -127 and up) with max|x| <= 448 * 2^e, so a code is x * 2^-e rounded to nearest
+ * even: off by at most 2^-4 of the value where that is at least 2^-6 * 2^e (2^-15 of the block's largest), by at most
+ * 2^-10 * 2^e below.  The product with the scale is exact.  inf and NaN are kept as NaN; they do not enter max|x|.  A
+ * block of zeros has s = 0.
  *   codes  : row r at codes + r * code_stride bytes (0: cols); bytes behind a row's last code are left alone
  *   scales : row r at scales + r * rlcu_act8_blocks(cols), one byte per block
  * Decoded values are rounded to the output's type once and, where they are finite, stay finite

@@ -140,6 +140,15 @@ int rlcu_preference_loss(const float* logp, uint64_t tokens, const float* ref_lo
                          const rlcu_preference_hparams* hp /* host */, float* coef, float* rewards,
                          rlcu_preference_stat* stat, uint32_t flags, void* stream);
 
+/* -------- bounded waits ------------------------------------------------------ */
+/* The CTAs that share a row of logits wait for one another, for a bounded time.  Waits for every stream of the
+ * device (cudaDeviceSynchronize) and reports whether such a wait gave up since the last check
+ * (RLCU_ERR_TIMEOUT: the results of that call are incomplete, the rows concerned are NaN).  Clears the condition. */
+int rlcu_losses_check(void);
+/* Runs a one-thread kernel whose bounded wait is certain to run out and reports it through the same path: the
+ * expected return value is RLCU_ERR_TIMEOUT, and the device stays usable. */
+int rlcu_losses_selftest_wait(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

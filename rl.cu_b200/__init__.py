@@ -45,6 +45,7 @@ EXPORTS = [
     "rlcu_zero1_step", "rlcu_zero1_poll_error", "rlcu_zero1_check", "rlcu_zero1_destroy",
     "rlcu_checkpoint_save", "rlcu_checkpoint_peek", "rlcu_checkpoint_load",
     "rlcu_token_logprob", "rlcu_token_logprob_grad", "rlcu_policy_loss", "rlcu_policy_loss_logp", "rlcu_preference_loss",
+    "rlcu_losses_check", "rlcu_losses_selftest_wait",
     "rlcu_act8_blocks", "rlcu_act8_store", "rlcu_act8_load", "rlcu_act8_rmsnorm", "rlcu_act8_rmsnorm_grad_workspace",
     "rlcu_act8_rmsnorm_grad",
 ]
@@ -206,6 +207,8 @@ def lib() -> C.CDLL:
     L.rlcu_policy_loss.argtypes = logits + [vp, vp, vp, vp, vp, vp, vp, vp, u64, vp, u32, vp]
     L.rlcu_policy_loss_logp.argtypes = [vp, u64, vp, vp, vp, vp, vp, vp, vp, u32, vp]
     L.rlcu_preference_loss.argtypes = [vp, u64, vp, vp, vp, u64, vp, vp, vp, vp, vp, u32, vp]
+    L.rlcu_losses_check.argtypes = []
+    L.rlcu_losses_selftest_wait.argtypes = [vp]
     L.rlcu_act8_blocks.argtypes = [u64]
     L.rlcu_act8_blocks.restype = u64
     L.rlcu_act8_store.argtypes = [vp, u32, u64, u64, u64, vp, u64, vp, vp]
@@ -460,6 +463,16 @@ def preference_loss(logp_ptr, tokens, offsets_ptr, pairs, hp: PreferenceHParams,
     """Preference loss of packed pairs of sequences; ``coef`` receives dloss/dlogp, ``rewards`` beta * s."""
     check(lib().rlcu_preference_loss(logp_ptr, tokens, ref_logp, mask, offsets_ptr, pairs, pair_weight, C.addressof(hp), coef,
                                      rewards, stat_ptr, flags, stream))
+
+
+def losses_check():
+    """Synchronise and raise if a bounded device-side wait of a loss kernel gave up."""
+    check(lib().rlcu_losses_check())
+
+
+def losses_selftest_wait(stream=None) -> int:
+    """Status of a wait that is certain to run out (``ERR_TIMEOUT``)."""
+    return lib().rlcu_losses_selftest_wait(stream)
 
 
 # ---------------------------------------------------------------------------

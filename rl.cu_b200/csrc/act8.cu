@@ -12,15 +12,6 @@
 #include "host_util.h"
 #include "typed.cuh"
 
-#ifndef GRAD_CTAS
-#define GRAD_CTAS (512 / THREADS)
-#endif
-#ifndef FWD_ROWS
-#define FWD_ROWS 8
-#endif
-#ifndef GRAD_PARTS
-#define GRAD_PARTS 296
-#endif
 namespace rlcu {
 namespace {
 
@@ -648,7 +639,7 @@ struct GradRow {
 };
 
 template <uint32_t DT, int TPR, int THREADS>
-__global__ void __launch_bounds__(THREADS, GRAD_CTAS)
+__global__ void __launch_bounds__(THREADS, 512 / THREADS)
 norm_grad_vec_kernel(NormArgs a) {
     using T = typename Elem<DT>::T;
     constexpr bool kAhead = DT != RLCU_F32;    // FP32 rows take twice the registers: two of them would spill
@@ -784,7 +775,7 @@ norm_weight_kernel(const float* partial, uint32_t parts, uint32_t cols, float* d
 // ---------------------------------------------------------------------------
 
 // CTAs the rows of a gradient are dealt to, at most: what the registers of 148 SMs hold of 256 threads each
-constexpr uint64_t kMostParts = GRAD_PARTS;
+constexpr uint64_t kMostParts = 2 * 148;
 
 uint64_t norm_parts(uint64_t rows) { return rows < kMostParts ? rows : kMostParts; }
 
@@ -830,7 +821,7 @@ constexpr uint64_t kMostVecCols = 8192;
 template <uint32_t DT, int TPR, int THREADS>
 int launch_norm_vec(const NormArgs& a, cudaStream_t s) {
     // a few rows per CTA, so that their weights are read once for them; the grid moves through memory in order
-    uint32_t per = THREADS / TPR * FWD_ROWS;
+    uint32_t per = THREADS / TPR * 8;
     while (per > THREADS / TPR * 2 && a.rows / per < 148 * 2048 / THREADS) per /= 2;
     norm_vec_kernel<DT, TPR, THREADS><<<(unsigned)((a.rows + per - 1) / per), THREADS, 0, s>>>(a, per);
     RLCU_CUDA(cudaGetLastError());

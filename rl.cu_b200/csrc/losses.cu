@@ -20,24 +20,6 @@ namespace {
 
 constexpr int kRowThreads = 512;
 constexpr float kLog2E = 1.4426950408889634f;
-#ifndef WIDE
-#define WIDE 256
-#endif
-#ifndef HELD_CTAS
-#define HELD_CTAS (1024 / THREADS)
-#endif
-#ifndef PREF_C
-#define PREF_C 16
-#endif
-#ifndef POL_C
-#define POL_C 8
-#endif
-#ifndef SUM_DEPTH
-#define SUM_DEPTH 4
-#endif
-#ifndef SUM_CTAS
-#define SUM_CTAS 1
-#endif
 constexpr float kLn2 = 0.6931471805599453f;
 // Where the running maximum starts: logits below it (-inf, and masks of a type's lowest value) add nothing,
 // and a row without any other has s = 0.
@@ -344,7 +326,6 @@ __device__ __forceinline__ void copy_async16(void* smem, const void* global) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
                  :: "r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(global) : "memory");
 }
-__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 constexpr int kMostCluster = 16;
 
@@ -390,9 +371,9 @@ constexpr uint32_t kWaitTries = 1u << 18;
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // bounded wait for a phase of an mbarrier of this CTA
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t phase) {
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t phase, uint32_t tries = kWaitTries) {
     uint32_t done = 0;
-    for (uint32_t i = 0; i < kWaitTries && !done; i++)
+    for (uint32_t i = 0; i < tries && !done; i++)
         asm volatile(
             "{\n"
             ".reg .pred p;\n"
@@ -518,7 +499,7 @@ struct RowFeed {
 // and keeps it in registers between the sum and the gradient: the logits are read once, the gradient is written once.
 // Several clusters share an SM, so that one row's loads and stores run under another's arithmetic.
 template <uint32_t DT, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, HELD_CTAS)
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
     using E = Elem<DT>;
     using T = typename E::T;
@@ -611,10 +592,10 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
 
 // Log-probabilities alone: a cluster (one CTA, unless rows are few) per row, kDepth groups per thread on their way in a
 // ring of slots.
-constexpr int kDepth = SUM_DEPTH;
+constexpr int kDepth = 4;
 
 template <uint32_t DT, int THREADS>
-__global__ void __launch_bounds__(THREADS, SUM_CTAS)
+__global__ void __launch_bounds__(THREADS)
 logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
     using E = Elem<DT>;
     extern __shared__ uint4 slots[];                  // [kDepth][THREADS]
@@ -733,14 +714,6 @@ struct PolicySums {
     uint32_t tokens = 0, clipped = 0;
     float ratio = 0.0f;
 
-    __device__ __forceinline__ void add(const PolicySums& o) {
-        l += o.l;
-        k += o.k;
-        w += o.w;
-        tokens += o.tokens;
-        clipped += o.clipped;
-        ratio = fmaxf(ratio, o.ratio);
-    }
     __device__ __forceinline__ void add_warp() {
 #pragma unroll
         for (int mask = 16; mask >= 1; mask >>= 1) {
@@ -764,6 +737,7 @@ policy_kernel(const float* logp, uint64_t tokens, const int32_t* targets, uint32
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ PolicySums warps[kVectorThreads / 32], ctas[kMostCluster];
     const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     PolicySums mine;
     for (uint64_t t = rank * kVectorThreads + threadIdx.x; t < tokens; t += C * kVectorThreads) {
         const float w = p.weight[t];
@@ -1014,6 +988,13 @@ preference_kernel(PreferenceArgs a) {
     }
 }
 
+// Waits for a barrier that nothing completes, as the kernels above would, with few tries.
+__global__ void wait_probe_kernel() {
+    __shared__ unsigned long long bar;
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(smem_at(&bar)) : "memory");
+    if (!wait_phase(smem_at(&bar), 0, 64)) atomicExch(&losses_error_word, 1u);
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -1108,7 +1089,7 @@ int launch_clusters(Kernel kernel, const LogitsArgs& a, const PolicyArgs& p, int
     return RLCU_OK;
 }
 
-constexpr int kWide = WIDE, kNarrow = 128, kMostHeld = 10;
+constexpr int kWide = 256, kNarrow = 128, kMostHeld = 10;
 
 template <uint32_t DT, int THREADS>
 int launch_policy_rows(const LogitsArgs& a, const PolicyArgs& p, int cluster, uint32_t held, cudaStream_t s) {
@@ -1168,11 +1149,16 @@ int launch_grad(const LogitsArgs& a, uint32_t dtype, const float* lse, const flo
     return RLCU_OK;
 }
 
+// behind: launched while the call's own kernel before it still runs (policy_kernel waits for its end)
 int launch_policy(const float* logp, uint64_t tokens, const int32_t* targets, uint32_t vocab, const PolicyArgs& p,
-                  float* coef, rlcu_policy_stat* stat, uint32_t flags, cudaStream_t s) {
-    if (POL_C > 8) RLCU_CUDA(cudaFuncSetAttribute(policy_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = cluster_launch(attr, tokens <= kVectorThreads ? 1 : tokens <= 4 * kVectorThreads ? 4 : POL_C, kVectorThreads, 0, s);
+                  float* coef, rlcu_policy_stat* stat, uint32_t flags, bool behind, cudaStream_t s) {
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = cluster_launch(attr, tokens <= kVectorThreads ? 1 : tokens <= 4 * kVectorThreads ? 4 : 8, kVectorThreads, 0, s);
+    if (behind) {
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 2;
+    }
     RLCU_CUDA(cudaLaunchKernelEx(&cfg, policy_kernel, logp, tokens, targets, vocab, p, coef, stat, flags));
     return RLCU_OK;
 }
@@ -1209,7 +1195,7 @@ extern "C" int rlcu_policy_loss_logp(const float* logp, uint64_t tokens, const f
     if (const int rc = check_policy(hp, ref_logp, advantage, weight, stat, tokens, flags)) return rc;
     if (tokens && !logp) return set_error(RLCU_ERR_INVALID, "null logp");
     PolicyArgs p = {old_logp, ref_logp, advantage, weight, *hp};
-    return launch_policy(logp, tokens, nullptr, 0, p, coef, stat, flags, (cudaStream_t)stream);
+    return launch_policy(logp, tokens, nullptr, 0, p, coef, stat, flags, false, (cudaStream_t)stream);
 }
 
 extern "C" int rlcu_policy_loss(const void* logits, uint32_t dtype, uint64_t rows, uint64_t vocab, uint64_t row_stride,
@@ -1229,7 +1215,7 @@ extern "C" int rlcu_policy_loss(const void* logits, uint32_t dtype, uint64_t row
                             : launch_logits<kModeLogprob>(a, p, dtype, (cudaStream_t)stream);
         if (rc) return rc;
     }
-    return launch_policy(logp, rows, targets, (uint32_t)vocab, p, nullptr, stat, flags, (cudaStream_t)stream);
+    return launch_policy(logp, rows, targets, (uint32_t)vocab, p, nullptr, stat, flags, rows > 0, (cudaStream_t)stream);
 }
 
 extern "C" int rlcu_preference_loss(const float* logp, uint64_t tokens, const float* ref_logp, const uint8_t* mask,
@@ -1251,10 +1237,25 @@ extern "C" int rlcu_preference_loss(const float* logp, uint64_t tokens, const fl
     PreferenceArgs a = {logp, ref_logp, mask, offsets, pair_weight, tokens, pairs, *hp, coef, rewards, stat, flags};
     // more CTAs than pairs would idle; below a few thousand tokens each, the cluster costs more than it saves
     int cluster = 1;
-    while (cluster < PREF_C && (uint64_t)cluster < pairs && tokens > (uint64_t)cluster * 4096) cluster *= 2;
+    while (cluster < kMostCluster && (uint64_t)cluster < pairs && tokens > (uint64_t)cluster * 4096) cluster *= 2;
     if (cluster > 8) RLCU_CUDA(cudaFuncSetAttribute(preference_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = cluster_launch(attr, cluster, kVectorThreads, 0, (cudaStream_t)stream);
     RLCU_CUDA(cudaLaunchKernelEx(&cfg, preference_kernel, a));
     return RLCU_OK;
+}
+
+extern "C" int rlcu_losses_check(void) {
+    RLCU_CUDA(cudaDeviceSynchronize());
+    unsigned int word = 0, none = 0;
+    RLCU_CUDA(cudaMemcpyFromSymbol(&word, losses_error_word, sizeof word));
+    if (!word) return RLCU_OK;
+    RLCU_CUDA(cudaMemcpyToSymbol(losses_error_word, &none, sizeof none));
+    return set_error(RLCU_ERR_TIMEOUT, "a bounded wait inside a loss kernel gave up: its results are incomplete");
+}
+
+extern "C" int rlcu_losses_selftest_wait(void* stream) {
+    wait_probe_kernel<<<1, 1, 0, (cudaStream_t)stream>>>();
+    RLCU_CUDA(cudaGetLastError());
+    return rlcu_losses_check();
 }

@@ -563,3 +563,67 @@ def test_captured_graph_follows_its_inputs(pkg):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(kept, (logp, stat, coef, grad)))
         assert float(grad.float().abs().sum()) > 0
+
+
+def test_bounded_waits_report_and_recover(pkg):
+    pkg.losses_check()
+    assert pkg.losses_selftest_wait() == pkg.ERR_TIMEOUT
+    pkg.losses_check()                                   # cleared, and the device is usable
+    check_policy(pkg, gaussian(20, 151936, "bf16", 5), targets_of(20, 151936, 5))
+    pkg.losses_check()
+
+
+def test_captured_policy_loss_follows_its_inputs(pkg):
+    """The fused call (rows taken over by clusters, the record from a dependent launch) captured once, replayed on other
+    contents, twice in a row."""
+    rows, vocab = 300, 32000
+    z, y = torch.empty(rows, vocab, dtype=torch.bfloat16, device="cuda"), torch.empty(rows, dtype=torch.int32, device="cuda")
+    a, w = torch.randn(rows, device="cuda"), torch.full((rows,), 1 / rows, device="cuda")
+    logp, grad, stat = torch.empty(rows, device="cuda"), torch.empty_like(z), torch.zeros(8, dtype=torch.int32, device="cuda")
+    hp = pkg.policy_hparams()
+
+    def call(stream):
+        pkg.policy_loss(z.data_ptr(), pkg.BF16, rows, vocab, y.data_ptr(), a.data_ptr(), w.data_ptr(), hp, logp.data_ptr(), grad.data_ptr(),
+                        stat.data_ptr(), stream=stream)
+
+    z.copy_(gaussian(rows, vocab, "bf16", 0))
+    y.copy_(targets_of(rows, vocab, 0))
+    call(None)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(torch.cuda.current_stream().cuda_stream)
+    for seed in (1, 2):
+        z.copy_(gaussian(rows, vocab, "bf16", seed))
+        y.copy_(targets_of(rows, vocab, seed))
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in (logp, stat, grad)]
+        for t in (logp, grad):
+            t.fill_(7)
+        call(None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(kept, (logp, stat, grad)))
+
+
+def test_policy_loss_reads_what_ran_before_it(pkg):
+    """Calls in a row on one stream, each on what the last one wrote: no launch may run ahead of the kernels it reads from."""
+    rows, vocab = 64, 4096
+    z0 = gaussian(rows, vocab, "f32", 3).cuda()
+    y, a, w = targets_of(rows, vocab, 3, 0.0).cuda(), torch.ones(rows, device="cuda"), torch.ones(rows, device="cuda")
+    hp = pkg.policy_hparams(1.0, math.inf)
+    results = []
+    for wait in (True, False):
+        z, logp, coef = z0.clone(), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+        stat, stat2 = (torch.zeros(8, dtype=torch.int32, device="cuda") for _ in range(2))
+        torch.cuda.synchronize()
+        for _ in range(30):
+            pkg.policy_loss(z.data_ptr(), pkg.F32, rows, vocab, y.data_ptr(), a.data_ptr(), w.data_ptr(), hp, logp.data_ptr(), z.data_ptr(), stat.data_ptr())
+            if wait:
+                torch.cuda.synchronize()
+            pkg.policy_loss_logp(logp.data_ptr(), rows, a.data_ptr(), w.data_ptr(), hp, stat2.data_ptr(), coef.data_ptr())
+            z.mul_(3.0).add_(z0)
+        torch.cuda.synchronize()
+        results.append((z, logp, coef, stat, stat2))
+    assert all(torch.equal(p, q) for p, q in zip(*results))
