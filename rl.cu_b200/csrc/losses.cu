@@ -472,7 +472,7 @@ struct RowFeed {
         asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
                      :: "r"(smem_at(&response)), "r"(smem_at(&bar)) : "memory");
     }
-    // first CTA of the cluster taken over by request n, or -1: none was left
+    // first CTA of the cluster taken over by request n (counted from 0), or -1: none was left
     __device__ __forceinline__ int answer(uint32_t n) {
         if (!wait_phase(smem_at(&bar), n & 1)) {
             atomicExch(&losses_error_word, 1u);
@@ -515,7 +515,7 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
     sums.init(C);
     uint32_t row = blockIdx.x / C;
     uint32_t y = row_takes_part(a, p, row, a.targets[row]) ? (uint32_t)a.targets[row] : kNoTarget;
-    for (uint32_t n = 0;; n++) {
+    for (uint32_t n = 0; n < a.rows; n++) {          // (rows do not run out of order twice: the bound is for safety)
         if (asks) feed.ask();
         const RowShare<DT, THREADS> now(a, row, y, rank, C);
         T* g = static_cast<T*>(a.grad) + (uint64_t)row * a.grad_stride;
@@ -590,21 +590,18 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
     sums.finish(C);
 }
 
-// Log-probabilities alone: a cluster (one CTA, unless rows are few) per row, kDepth groups per thread on their way in a
-// ring of slots.
-constexpr int kDepth = 4;
+// Log-probabilities alone: a cluster (one CTA, unless rows are few) per row, kDepth groups per thread on their way.
+constexpr int kDepth = 5;
 
 template <uint32_t DT, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
     using E = Elem<DT>;
-    extern __shared__ uint4 slots[];                  // [kDepth][THREADS]
     __shared__ ClusterSum<THREADS / 32> sums;
     __shared__ float z_y;
     const uint32_t C = cooperative_groups::this_cluster().num_blocks(), rank = cooperative_groups::this_cluster().block_rank();
     const int tid = threadIdx.x;
     const float c = a.inv_temperature * kLog2E;
-    uint4* mine = slots + tid;
     const uint32_t row = blockIdx.x / C;
     const int32_t y = a.targets[row];
     if (!row_takes_part(a, p, row, y)) {              // (the whole cluster)
@@ -615,27 +612,26 @@ logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
         return;
     }
     const RowShare<DT, THREADS> now(a, row, (uint32_t)y, rank, C);
+    uint4 next[kDepth];
 #pragma unroll
-    for (int d = 0; d < kDepth; d++) {
-        if ((uint32_t)d < now.groups) copy_async16(mine + d * THREADS, now.in + d * THREADS);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+    for (int d = 0; d < kDepth; d++)
+        if ((uint32_t)d < now.groups) next[d] = __ldcs(now.in + d * THREADS);
     float end = 0.0f;
     if (now.end_at < a.vocab) end = E::up(now.x[now.end_at]);
     if (tid == 32) z_y = E::up(now.x[y]);
     sums.init(C);
     Online o(c);
     const uint4* in = now.in + kDepth * THREADS;
-    for (uint32_t j0 = 0; j0 < now.groups; j0 += kDepth) {
+    for (uint32_t j = 0; j < now.groups; j += kDepth) {
+        uint4 v[kDepth];
 #pragma unroll
         for (int d = 0; d < kDepth; d++) {
-            if (j0 + d < now.groups) {
-                asm volatile("cp.async.wait_group %0;" :: "n"(kDepth - 1) : "memory");
-                o.add<DT>(mine[d * THREADS], c);
-                if (j0 + d + kDepth < now.groups) copy_async16(mine + d * THREADS, in + d * THREADS);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            }
+            v[d] = next[d];
+            if (j + kDepth + d < now.groups) next[d] = __ldcs(in + d * THREADS);
         }
+#pragma unroll
+        for (int d = 0; d < kDepth; d++)
+            if (j + d < now.groups) o.add<DT>(v[d], c);
         in += kDepth * THREADS;
     }
     if (now.end_at < a.vocab) o.add(end, c);
@@ -1115,8 +1111,8 @@ int launch_logits_dt(const LogitsArgs& a, const PolicyArgs& p, int sms, uint64_t
         const uint32_t held = (uint32_t)(((groups + cluster - 1) / cluster + threads - 1) / threads);
         return threads == kWide ? launch_policy_rows<DT, kWide>(a, p, cluster, held, s) : launch_policy_rows<DT, kNarrow>(a, p, cluster, held, s);
     }
-    return threads == 256 ? launch_clusters(logits_sum_kernel<DT, 256>, a, p, cluster, 256, kDepth * 256 * 16, s)
-                          : launch_clusters(logits_sum_kernel<DT, kNarrow>, a, p, cluster, kNarrow, kDepth * kNarrow * 16, s);
+    return threads == 256 ? launch_clusters(logits_sum_kernel<DT, 256>, a, p, cluster, 256, 0, s)
+                          : launch_clusters(logits_sum_kernel<DT, kNarrow>, a, p, cluster, kNarrow, 0, s);
 }
 
 // every row of the gradient starts at the same place of a 16-byte group as its logits do

@@ -146,6 +146,15 @@ def test_logprob_masked_logits(pkg, dtype, vocab):
     check_logprob(pkg, z, y)
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [(6000, 600, "f16"), (9001, 515, "f32"), (2500, 9000, "bf16"), (1500, 16411, "f16"), (260, 151936, "bf16")])
+def test_rows_by_the_thousand(pkg, rows, vocab, dtype):
+    """More rows than fit the GPU at once: CTAs and clusters take over row after row, each exactly once."""
+    z, y = gaussian(rows, vocab, dtype, rows), targets_of(rows, vocab, rows)
+    check_logprob(pkg, z, y)
+    check_policy(pkg, z, y, scale=64.0)
+    pkg.losses_check()
+
+
 def test_logprob_huge_logits_do_not_vanish(pkg):
     z = torch.full((2, 64), 3.0e38, dtype=torch.float32)
     logp, _, _ = run_logprob(pkg, z, torch.tensor([0, 1], dtype=torch.int32), 1.0)
