@@ -53,36 +53,48 @@ __device__ __forceinline__ float keep_finite(float v) {
     return fabsf(v) > most ? copysignf(most, v) : v;
 }
 
-// One warp per block of 128 columns.
+// Element by element, for rows that start anywhere: a warp per kWarpBlocks blocks of a row, lane i with every 32nd column,
+// all of its loads in flight at once.
+constexpr int kWarpBlocks = 4, kPerLane = kWarpBlocks * (int)kBlock / 32;
+
+// where the calling warp works: false if there is nothing
+__device__ __forceinline__ bool warp_place(uint64_t rows, uint32_t blocks, uint64_t& row, uint32_t& block) {
+    const uint32_t per_row = (blocks + kWarpBlocks - 1) / kWarpBlocks;
+    const uint64_t unit = (uint64_t)blockIdx.x * (kAct8Threads / 32) + (threadIdx.x >> 5);
+    row = unit <= 0xFFFFFFFFull ? (uint32_t)unit / per_row : unit / per_row;
+    block = (uint32_t)(unit - row * per_row) * kWarpBlocks;
+    return row < rows;
+}
+
 template <uint32_t DT>
 __global__ void __launch_bounds__(kAct8Threads)
 act8_store_kernel(const void* x, uint64_t rows, uint32_t cols, uint64_t x_stride, uint8_t* codes, uint64_t code_stride,
                   uint8_t* scales) {
     using E = Elem<DT>;
-    const uint32_t blocks = (cols + kBlock - 1) / kBlock;
-    const uint64_t total = rows * blocks, step = (uint64_t)gridDim.x * (kAct8Threads / 32);
-    const uint32_t lane = threadIdx.x & 31;
-    for (uint64_t b = (uint64_t)blockIdx.x * (kAct8Threads / 32) + (threadIdx.x >> 5); b < total; b += step) {
-        const uint64_t row = b / blocks;
-        const uint32_t col = (uint32_t)(b - row * blocks) * kBlock;
-        const typename E::T* in = static_cast<const typename E::T*>(x) + row * x_stride;
-        float v[4], top = 0.0f;
+    const uint32_t blocks = (cols + kBlock - 1) / kBlock, lane = threadIdx.x & 31;
+    uint64_t row;
+    uint32_t block;
+    if (!warp_place(rows, blocks, row, block)) return;
+    const uint32_t col = block * kBlock + lane;
+    const typename E::T* in = static_cast<const typename E::T*>(x) + row * x_stride + col;
+    uint8_t* out = codes + row * code_stride + col;
+    float v[kPerLane];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t j = col + i * 32 + lane;
-            v[i] = j < cols ? E::up(in[j]) : 0.0f;
+    for (int i = 0; i < kPerLane; i++) v[i] = col + i * 32 < cols ? E::up(in[i * 32]) : 0.0f;
+#pragma unroll
+    for (int b = 0; b < kWarpBlocks; b++) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 4 * b; i < 4 * b + 4; i++)
             if (fabsf(v[i]) <= FLT_MAX) top = fmaxf(top, fabsf(v[i]));
-        }
 #pragma unroll
         for (int mask = 16; mask >= 1; mask >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, mask));
         const uint32_t byte = scale_byte(top);
         const float inv = pow2(127 - (int)byte);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t j = col + i * 32 + lane;
-            if (j < cols) codes[row * code_stride + j] = encode(v[i], inv);
-        }
-        if (lane == 0) scales[b] = (uint8_t)byte;
+        for (int i = 4 * b; i < 4 * b + 4; i++)
+            if (col + i * 32 < cols) out[i * 32] = encode(v[i], inv);
+        if (lane == 0 && block + b < blocks) scales[row * blocks + block + b] = (uint8_t)byte;
     }
 }
 
@@ -91,20 +103,21 @@ __global__ void __launch_bounds__(kAct8Threads)
 act8_load_kernel(const uint8_t* codes, uint64_t code_stride, const uint8_t* scales, uint64_t rows, uint32_t cols, void* x,
                  uint64_t x_stride) {
     using E = Elem<DT>;
-    const uint32_t blocks = (cols + kBlock - 1) / kBlock;
-    const uint64_t total = rows * blocks, step = (uint64_t)gridDim.x * (kAct8Threads / 32);
-    const uint32_t lane = threadIdx.x & 31;
-    for (uint64_t b = (uint64_t)blockIdx.x * (kAct8Threads / 32) + (threadIdx.x >> 5); b < total; b += step) {
-        const uint64_t row = b / blocks;
-        const uint32_t col = (uint32_t)(b - row * blocks) * kBlock;
-        typename E::T* out = static_cast<typename E::T*>(x) + row * x_stride;
-        const float scale = pow2((int)scales[b] - 127);
+    const uint32_t blocks = (cols + kBlock - 1) / kBlock, lane = threadIdx.x & 31;
+    uint64_t row;
+    uint32_t block;
+    if (!warp_place(rows, blocks, row, block)) return;
+    const uint32_t col = block * kBlock + lane;
+    const uint8_t* in = codes + row * code_stride + col;
+    typename E::T* out = static_cast<typename E::T*>(x) + row * x_stride + col;
+    uint8_t v[kPerLane], byte[kWarpBlocks];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t j = col + i * 32 + lane;
-            if (j < cols) out[j] = E::down(keep_finite<DT>(decode(codes[row * code_stride + j], scale)));
-        }
-    }
+    for (int i = 0; i < kPerLane; i++) v[i] = col + i * 32 < cols ? in[i * 32] : 0;
+#pragma unroll
+    for (int b = 0; b < kWarpBlocks; b++) byte[b] = block + b < blocks ? scales[row * blocks + block + b] : 0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; i++)
+        if (col + i * 32 < cols) out[i * 32] = E::down(keep_finite<DT>(decode(v[i], pow2((int)byte[i / 4] - 127))));
 }
 
 // The same in 16-byte accesses, for rows that start on 16-byte boundaries: eight threads per block of 128, 16 columns
@@ -406,7 +419,7 @@ __device__ __forceinline__ float2 block_sum2(float x, float y, float2* smem) {
     return make_float2(x, y);
 }
 
-// One CTA per row at a time, the row decoded twice: any width.
+// One CTA per row at a time, the row decoded twice: rows wider than the kernels below hold.
 template <uint32_t DT>
 __global__ void __launch_bounds__(kAct8Threads)
 norm_kernel(NormArgs a) {
@@ -475,8 +488,16 @@ struct RowSum {
         if constexpr (TPR > 32) {
             const uint32_t warp = threadIdx.x >> 5, group = threadIdx.x / TPR;
             if ((threadIdx.x & 31) == 0) part[step & 1][warp] = make_float2(x, y);
-            if constexpr (TPR == THREADS) __syncthreads();
-            else asm volatile("barrier.cta.sync %0, %1;" :: "r"(group + 1), "n"(TPR) : "memory");
+            if constexpr (TPR == THREADS) {
+                __syncthreads();
+            } else {
+                // each group its own barrier, by constant numbers (a number in a register would claim all sixteen)
+                static_assert(THREADS / TPR <= 4, "barriers");
+                if (group == 0) asm volatile("barrier.cta.sync 1, %0;" :: "n"(TPR) : "memory");
+                else if (group == 1) asm volatile("barrier.cta.sync 2, %0;" :: "n"(TPR) : "memory");
+                else if (group == 2) asm volatile("barrier.cta.sync 3, %0;" :: "n"(TPR) : "memory");
+                else asm volatile("barrier.cta.sync 4, %0;" :: "n"(TPR) : "memory");
+            }
             x = y = 0.0f;
 #pragma unroll
             for (int w = 0; w < TPR / 32; w++) {
@@ -747,6 +768,127 @@ norm_grad_vec_kernel(NormArgs a) {
     }
 }
 
+// Rows that start anywhere: thread t of the TPR that have a row takes columns t, t + TPR, ..., kColumns at most, one
+// element per access (a warp's 32 are side by side).
+constexpr int kColumns = 8;
+
+// one code without its scale
+__device__ __forceinline__ float code_value(uint8_t code) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)code));
+    return __half2float(__ushort_as_half((uint16_t)h));
+}
+
+// A thread's columns of one row: codes, and the scales of the blocks they lie in.
+template <int TPR>
+struct Columns {
+    uint8_t code[kColumns], byte[kColumns];
+
+    __device__ __forceinline__ Columns(const NormArgs& a, uint32_t row, uint32_t lane) {
+        const uint8_t* c = a.codes + row * a.code_stride + lane;
+        const uint8_t* s = a.scales + (uint64_t)row * a.blocks + lane / kBlock;
+#pragma unroll
+        for (int k = 0; k < kColumns; k++) {
+            const bool in = lane + k * TPR < a.cols;
+            code[k] = in ? c[k * TPR] : 0;
+            byte[k] = in ? s[k * TPR / (int)kBlock] : 0;          // TPR = 32: a warp's columns lie in one block
+        }
+    }
+    __device__ __forceinline__ float scale(int k) const { return pow2((int)byte[k] - 127); }
+};
+
+template <uint32_t DT, int TPR, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+norm_col_kernel(NormArgs a, uint32_t rows_per_cta) {
+    using E = Elem<DT>;
+    __shared__ RowSum<TPR, THREADS> sum;
+    const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows;
+    const uint32_t first = blockIdx.x * rows_per_cta + threadIdx.x / TPR, last = min(rows, (blockIdx.x + 1) * rows_per_cta);
+    float w[kColumns];
+#pragma unroll
+    for (int k = 0; k < kColumns; k++) w[k] = lane + k * TPR < a.cols ? weight_at(a, lane + k * TPR) : 0.0f;
+    uint32_t step = 0;
+    for (uint32_t row = first; row < last; row += THREADS / TPR, step++) {
+        const Columns<TPR> x(a, row, lane);
+        float c[kColumns], sq = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kColumns; k++) {
+            c[k] = code_value(x.code[k]);
+            const float v = c[k] * x.scale(k);
+            sq = fmaf(v, v, sq);
+        }
+        const float rstd = 1.0f / sqrtf(sum(sq, 0.0f, step).x / (float)a.cols + a.eps);
+        if (a.rstd && lane == 0) a.rstd[row] = rstd;
+        typename E::T* out = static_cast<typename E::T*>(a.out) + row * a.out_stride + lane;
+#pragma unroll
+        for (int k = 0; k < kColumns; k++)
+            if (lane + k * TPR < a.cols) out[k * TPR] = E::down(c[k] * (x.scale(k) * rstd) * w[k]);
+    }
+}
+
+template <uint32_t DT, int TPR, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS <= 256 ? 3 : THREADS <= 512 ? 2 : 1)
+norm_grad_col_kernel(NormArgs a) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    __shared__ RowSum<TPR, THREADS> sum;
+    const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows, at_once = THREADS / TPR, jump = gridDim.x * at_once;
+    float w[kColumns], dw[kColumns];
+#pragma unroll
+    for (int k = 0; k < kColumns; k++) {
+        w[k] = lane + k * TPR < a.cols ? weight_at(a, lane + k * TPR) : 0.0f;
+        dw[k] = 0.0f;
+    }
+    uint32_t step = 0;
+    for (uint32_t row = blockIdx.x * at_once + threadIdx.x / TPR; row < rows; row += jump, step++) {
+        const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride + lane;
+        const T* dres = static_cast<const T*>(a.dres) + row * a.dres_stride + lane;
+        T* out = static_cast<T*>(a.out) + row * a.out_stride + lane;
+        const Columns<TPR> x(a, row, lane);
+        T d[kColumns], r[kColumns];
+#pragma unroll
+        for (int k = 0; k < kColumns; k++) {
+            const bool in = lane + k * TPR < a.cols;
+            d[k] = in ? dy[k * TPR] : (T)0;
+            r[k] = in && a.dres ? dres[k * TPR] : (T)0;
+        }
+        float sq = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kColumns; k++) {
+            const float v = code_value(x.code[k]) * x.scale(k);
+            sq = fmaf(v, v, sq);
+            dot = fmaf(E::up(d[k]) * w[k], v, dot);
+        }
+        const float2 sums = sum(sq, dot, step);
+        const float rstd = 1.0f / sqrtf(sums.x / (float)a.cols + a.eps);
+        const float pull = sums.y / (float)a.cols * rstd * rstd;
+#pragma unroll
+        for (int k = 0; k < kColumns; k++) {
+            if (lane + k * TPR >= a.cols) continue;
+            const float c = code_value(x.code[k]), s = x.scale(k), dk = E::up(d[k]);
+            dw[k] = fmaf(dk, c * (s * rstd), dw[k]);
+            out[k * TPR] = E::down(fmaf(rstd, fmaf(-c, s * pull, dk * w[k]), a.dres ? E::up(r[k]) : 0.0f));
+        }
+    }
+    if (!a.partial) return;
+    float* part = a.partial + (uint64_t)blockIdx.x * a.cols;
+    if constexpr (TPR < THREADS) {
+        // the CTA's groups have the same columns: the first to the last, in turn
+        __shared__ float shared[TPR * kColumns];
+        for (int turn = 0; turn < (int)at_once; turn++) {
+            if (threadIdx.x / TPR == turn)
+#pragma unroll
+                for (int k = 0; k < kColumns; k++) shared[lane + k * TPR] = turn ? shared[lane + k * TPR] + dw[k] : dw[k];
+            __syncthreads();
+        }
+        for (uint32_t j = threadIdx.x; j < a.cols; j += THREADS) part[j] = shared[j];
+    } else {
+#pragma unroll
+        for (int k = 0; k < kColumns; k++)
+            if (lane + k * TPR < a.cols) part[lane + k * TPR] = dw[k];
+    }
+}
+
 // dweight from the CTAs' partial sums: a CTA per 32 columns, each warp every 32nd part, then the warps in order.  Launched
 // while the gradient kernel still runs; it waits for its end.
 constexpr int kWeightThreads = 1024;
@@ -828,6 +970,15 @@ int launch_norm_vec(const NormArgs& a, cudaStream_t s) {
     return RLCU_OK;
 }
 
+template <uint32_t DT, int TPR, int THREADS>
+int launch_norm_col(const NormArgs& a, cudaStream_t s) {
+    uint32_t per = THREADS / TPR * 8;
+    while (per > THREADS / TPR && a.rows / per < 148 * 2048 / THREADS) per /= 2;
+    norm_col_kernel<DT, TPR, THREADS><<<(unsigned)((a.rows + per - 1) / per), THREADS, 0, s>>>(a, per);
+    RLCU_CUDA(cudaGetLastError());
+    return RLCU_OK;
+}
+
 template <uint32_t DT>
 int launch_norm(const NormArgs& a, bool vec, cudaStream_t s) {
     if (vec) {
@@ -837,6 +988,10 @@ int launch_norm(const NormArgs& a, bool vec, cudaStream_t s) {
         if (a.cols <= 4096) return launch_norm_vec<DT, 256, 256>(a, s);
         return launch_norm_vec<DT, 512, 512>(a, s);
     }
+    if (a.cols <= 32 * kColumns) return launch_norm_col<DT, 32, 256>(a, s);
+    if (a.cols <= 128 * kColumns) return launch_norm_col<DT, 128, 256>(a, s);
+    if (a.cols <= 512 * kColumns) return launch_norm_col<DT, 512, 512>(a, s);
+    if (a.cols <= 1024 * kColumns) return launch_norm_col<DT, 1024, 1024>(a, s);
     int grid = 0;
     if (const int rc = grid_for(a.rows, 8, &grid)) return rc;
     norm_kernel<DT><<<grid, kAct8Threads, 0, s>>>(a);
@@ -853,6 +1008,15 @@ int launch_norm_grad_vec(const NormArgs& a, int* parts, cudaStream_t s) {
     return RLCU_OK;
 }
 
+template <uint32_t DT, int TPR, int THREADS>
+int launch_norm_grad_col(const NormArgs& a, int* parts, cudaStream_t s) {
+    const uint64_t at_once = THREADS / TPR, steps = (a.rows + at_once - 1) / at_once;
+    *parts = (int)norm_parts(steps);
+    norm_grad_col_kernel<DT, TPR, THREADS><<<*parts, THREADS, 0, s>>>(a);
+    RLCU_CUDA(cudaGetLastError());
+    return RLCU_OK;
+}
+
 template <uint32_t DT>
 int launch_norm_grad(const NormArgs& a, bool vec, int* parts, cudaStream_t s) {
     if (vec) {
@@ -862,6 +1026,10 @@ int launch_norm_grad(const NormArgs& a, bool vec, int* parts, cudaStream_t s) {
         if (a.cols <= 4096) return launch_norm_grad_vec<DT, 256, 256>(a, parts, s);
         return launch_norm_grad_vec<DT, 512, 512>(a, parts, s);
     }
+    if (a.cols <= 32 * kColumns) return launch_norm_grad_col<DT, 32, 256>(a, parts, s);
+    if (a.cols <= 128 * kColumns) return launch_norm_grad_col<DT, 128, 256>(a, parts, s);
+    if (a.cols <= 512 * kColumns) return launch_norm_grad_col<DT, 512, 512>(a, parts, s);
+    if (a.cols <= 1024 * kColumns) return launch_norm_grad_col<DT, 1024, 1024>(a, parts, s);
     *parts = (int)norm_parts(a.rows);
     norm_grad_kernel<DT><<<*parts, kAct8Threads, 0, s>>>(a);
     RLCU_CUDA(cudaGetLastError());
@@ -894,8 +1062,9 @@ extern "C" int rlcu_act8_store(const void* x, uint32_t dtype, uint64_t rows, uin
         else RLCU_STORE(RLCU_F32);
 #undef RLCU_STORE
     } else {
-        int grid = 0;
-        if (const int rc = grid_for((total + 7) / 8, 8, &grid)) return rc;
+        const uint64_t warps = rows * ((blocks + kWarpBlocks - 1) / kWarpBlocks), ctas = (warps + kAct8Threads / 32 - 1) / (kAct8Threads / 32);
+        if (ctas > 0x7FFFFFFFull) return set_error(RLCU_ERR_INVALID, "too many rows for rows that are not 16-byte aligned");
+        const unsigned grid = (unsigned)ctas;
         if (dtype == RLCU_F16) act8_store_kernel<RLCU_F16><<<grid, kAct8Threads, 0, s>>>(x, rows, (uint32_t)cols, x_stride, codes, code_stride, scales);
         else if (dtype == RLCU_BF16) act8_store_kernel<RLCU_BF16><<<grid, kAct8Threads, 0, s>>>(x, rows, (uint32_t)cols, x_stride, codes, code_stride, scales);
         else act8_store_kernel<RLCU_F32><<<grid, kAct8Threads, 0, s>>>(x, rows, (uint32_t)cols, x_stride, codes, code_stride, scales);
@@ -921,8 +1090,9 @@ extern "C" int rlcu_act8_load(const uint8_t* codes, uint64_t code_stride, const 
         else RLCU_LOAD(RLCU_F32);
 #undef RLCU_LOAD
     } else {
-        int grid = 0;
-        if (const int rc = grid_for((total + 7) / 8, 8, &grid)) return rc;
+        const uint64_t warps = rows * ((blocks + kWarpBlocks - 1) / kWarpBlocks), ctas = (warps + kAct8Threads / 32 - 1) / (kAct8Threads / 32);
+        if (ctas > 0x7FFFFFFFull) return set_error(RLCU_ERR_INVALID, "too many rows for rows that are not 16-byte aligned");
+        const unsigned grid = (unsigned)ctas;
         if (dtype == RLCU_F16) act8_load_kernel<RLCU_F16><<<grid, kAct8Threads, 0, s>>>(codes, code_stride, scales, rows, (uint32_t)cols, x, x_stride);
         else if (dtype == RLCU_BF16) act8_load_kernel<RLCU_BF16><<<grid, kAct8Threads, 0, s>>>(codes, code_stride, scales, rows, (uint32_t)cols, x, x_stride);
         else act8_load_kernel<RLCU_F32><<<grid, kAct8Threads, 0, s>>>(codes, code_stride, scales, rows, (uint32_t)cols, x, x_stride);
