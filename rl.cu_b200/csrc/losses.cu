@@ -233,8 +233,9 @@ __device__ __forceinline__ void zero_row(void* grad, uint64_t at, uint32_t vocab
     for (uint32_t i = cut.head + cut.groups * E::kVec + tid; i < vocab; i += threads) out[i] = E::down(0.0f);
 }
 
-// One CTA per row, two passes: the running sum, then the gradient.  The second pass finds the row in L2 (148
-// rows of 300 KB are 44 MB of its 126).
+// One CTA per row, two passes: the running sum, then the gradient.  For what the kernels below do not take: a gradient
+// whose rows lie at other 16-byte offsets than the logits', vocabularies of less than 64 groups of 16 bytes, rows beyond
+// sixteen CTAs' registers.  4096 x 151936 bf16 takes 627 us this way.
 template <uint32_t DT, int MODE>
 __global__ void __launch_bounds__(kRowThreads)
 logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* coef_in) {
@@ -322,11 +323,7 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
     }
 }
 
-__device__ __forceinline__ void copy_async16(void* smem, const void* global) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                 :: "r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(global) : "memory");
-}
-
+// CTAs that may share a row or a record.  More than 8 need the kernel's consent (non-portable cluster size).
 constexpr int kMostCluster = 16;
 
 // A row's share of one thread of a CTA: every THREADS-th group of the CTA's run, and perhaps one of the single
@@ -386,8 +383,8 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t phase, uint32_
 
 // Sums of all threads of a cluster, in warp 0 of each of its CTAs.  The CTAs hand each other their sums with st.async,
 // whose arrival the receiver's mbarrier counts in bytes: unlike a cluster barrier with release semantics this does not
-// wait for the gradient stores that are still on their way (which took longer than the row's arithmetic: 667 us
-// instead of ~ for 4096 x 151936 bf16).
+// wait for the gradient stores that are still on their way (an earlier form of the policy kernel took 667 us with the
+// barrier and 629 us with this, 4096 x 151936 bf16).
 template <int WARPS>
 struct ClusterSum {
     float2 part[2][kMostCluster * WARPS];  // (e, s) of each warp of the cluster, by row parity: a CTA may be a row ahead
@@ -497,7 +494,15 @@ struct RowFeed {
 
 // The policy loss of most calls.  A row belongs to a cluster of C CTAs, each of which has a run of its 16-byte groups
 // and keeps it in registers between the sum and the gradient: the logits are read once, the gradient is written once.
-// Several clusters share an SM, so that one row's loads and stores run under another's arithmetic.
+// Several clusters share an SM (four CTAs of 256 threads with up to ten groups each: 160 KB of its registers), so that
+// one row's loads and stores run under another's arithmetic.
+// Measured (B200, a tenth of the rows without part): 4096 x 151936 bf16 464 us, 0.78 of the copy rate (6.55 TB/s) for the
+// bytes it cannot do without; 1000 x 151936 f32 229 us, 0.81.  A row takes a CTA about 14,500 cycles: 3,500 until its loads
+// are there, 3,000 for the sum, 3,000 to 4,500 to exchange it, 1,100 for the row's factors, 2,000 for the gradient; with
+// four CTAs per SM the special-function units and the issue slots are each a little over half busy.  The same kernel
+// without any arithmetic takes 421 us, a plain copy of the same bytes 335 us.  Fetching the next row ahead (into L2, into
+// shared memory by cp.async or by a bulk copy), a second row in the same loop, and five or six CTAs per SM with part of
+// the row in shared memory were all slower (453 to 720 us; L2 prefetch gained 2 % here and lost 20 % for f32).
 template <uint32_t DT, int THREADS, int NV>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
@@ -515,7 +520,7 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
     sums.init(C);
     uint32_t row = blockIdx.x / C;
     uint32_t y = row_takes_part(a, p, row, a.targets[row]) ? (uint32_t)a.targets[row] : kNoTarget;
-    for (uint32_t n = 0; n < a.rows; n++) {          // (rows do not run out of order twice: the bound is for safety)
+    for (uint32_t n = 0; n < a.rows; n++) {          // (ends at the break; the bound holds whatever the feed answers)
         if (asks) feed.ask();
         const RowShare<DT, THREADS> now(a, row, y, rank, C);
         T* g = static_cast<T*>(a.grad) + (uint64_t)row * a.grad_stride;
@@ -590,7 +595,9 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
     sums.finish(C);
 }
 
-// Log-probabilities alone: a cluster (one CTA, unless rows are few) per row, kDepth groups per thread on their way.
+// Log-probabilities alone: a cluster (one CTA, unless rows are few) per row, kDepth groups per thread on their way in
+// registers.  Bound by HBM: 2048 x 151936 bf16 97 us, 0.88 of the copy rate; the same with the groups on their way by
+// cp.async through shared memory 106 us, with CTAs that stay and take over rows 110 us.
 constexpr int kDepth = 5;
 
 template <uint32_t DT, int THREADS>
@@ -649,7 +656,8 @@ logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
 }
 
 // The gradient alone (the sum is known): elementwise, a CTA per run of kGradGroups groups of a row, so that the grid
-// moves through memory in order.
+// moves through memory in order.  Bound by HBM: with the sum before it, 1000 x 50001 f32 97 us for 560 MB (the logits
+// are read twice), 0.88 of the copy rate.
 constexpr int kGradThreads = 256, kGradPer = 4, kGradGroups = kGradThreads * kGradPer;
 
 template <uint32_t DT>
@@ -725,7 +733,7 @@ struct PolicySums {
 
 // Weighted sums of the policy loss over all tokens, and the gradient by log-probability.  `targets` (with vocab):
 // tokens whose target is out of range take no part.  One cluster: its CTAs hand their sums to the first one, so the
-// record needs no scratch memory and no second launch.
+// record needs no scratch memory and no second launch.  Bound by latency: 16384 tokens 4.5 us in a graph.
 __global__ void __launch_bounds__(kVectorThreads)
 policy_kernel(const float* logp, uint64_t tokens, const int32_t* targets, uint32_t vocab, PolicyArgs p, float* coef,
               rlcu_policy_stat* stat, uint32_t flags) {
@@ -824,7 +832,8 @@ __device__ __forceinline__ void preference_term(const rlcu_preference_hparams& h
 
 // One cluster, so that the record needs no scratch memory and no second launch.  CTA r has the pairs r, r + C, ... and
 // works on kBatch of them at a time, whatever their lengths: their tokens are cut into at most kSegments segments of
-// equal length, a warp sums a segment, and the segments of a sequence are added in order.
+// equal length, a warp sums a segment, and the segments of a sequence are added in order.  Bound by latency and by what 16
+// SMs read: 128 pairs of 2048 tokens 16 us (a CTA per pair in turn: 706 us), one pair of 200 6 us in a graph.
 constexpr int kBatch = 16, kSegments = 512;
 
 __global__ void __launch_bounds__(kVectorThreads)
@@ -1060,14 +1069,13 @@ int launch_rows(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, const 
 }
 
 // one cluster of `cluster` CTAs
-cudaLaunchConfig_t cluster_launch(cudaLaunchAttribute* attr, int cluster, int threads, int smem, cudaStream_t s) {
+cudaLaunchConfig_t cluster_launch(cudaLaunchAttribute* attr, int cluster, int threads, cudaStream_t s) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cluster);
     cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -1075,11 +1083,10 @@ cudaLaunchConfig_t cluster_launch(cudaLaunchAttribute* attr, int cluster, int th
 }
 
 template <typename Kernel>
-int launch_clusters(Kernel kernel, const LogitsArgs& a, const PolicyArgs& p, int cluster, int threads, int smem, cudaStream_t s) {
-    RLCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+int launch_clusters(Kernel kernel, const LogitsArgs& a, const PolicyArgs& p, int cluster, int threads, cudaStream_t s) {
     if (cluster > 8) RLCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = cluster_launch(attr, cluster, threads, smem, s);
+    cudaLaunchConfig_t cfg = cluster_launch(attr, cluster, threads, s);
     cfg.gridDim = dim3((unsigned)(a.rows * cluster));
     RLCU_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, p));
     return RLCU_OK;
@@ -1090,7 +1097,7 @@ constexpr int kWide = 256, kNarrow = 128, kMostHeld = 10;
 template <uint32_t DT, int THREADS>
 int launch_policy_rows(const LogitsArgs& a, const PolicyArgs& p, int cluster, uint32_t held, cudaStream_t s) {
 #define RLCU_HELD(NV) \
-    if (held <= NV) return launch_clusters(logits_policy_kernel<DT, THREADS, NV>, a, p, cluster, THREADS, 0, s)
+    if (held <= NV) return launch_clusters(logits_policy_kernel<DT, THREADS, NV>, a, p, cluster, THREADS, s)
     RLCU_HELD(2);
     RLCU_HELD(4);
     RLCU_HELD(6);
@@ -1102,17 +1109,19 @@ int launch_policy_rows(const LogitsArgs& a, const PolicyArgs& p, int cluster, ui
 
 template <uint32_t DT, int MODE>
 int launch_logits_dt(const LogitsArgs& a, const PolicyArgs& p, int sms, uint64_t groups, cudaStream_t s) {
-    const int threads = MODE == kModePolicy ? (groups > kNarrow * kMostHeld ? kWide : kNarrow) : (groups > 1024 ? 256 : kNarrow);
+    // a row of up to kNarrow * kMostHeld groups fits one narrow CTA, and twice as many rows an SM
+    const int threads = groups > (MODE == kModePolicy ? kNarrow * kMostHeld : 1024) ? kWide : kNarrow;
     int cluster = 1;
     if (MODE == kModePolicy)
         while (cluster < kMostCluster && groups > (uint64_t)cluster * threads * kMostHeld) cluster *= 2;
+    // few rows: spread each over more SMs, as long as every thread keeps a group
     while (cluster < 8 && a.rows * cluster < (uint64_t)sms && groups > (uint64_t)cluster * threads) cluster *= 2;
     if (MODE == kModePolicy) {
         const uint32_t held = (uint32_t)(((groups + cluster - 1) / cluster + threads - 1) / threads);
         return threads == kWide ? launch_policy_rows<DT, kWide>(a, p, cluster, held, s) : launch_policy_rows<DT, kNarrow>(a, p, cluster, held, s);
     }
-    return threads == 256 ? launch_clusters(logits_sum_kernel<DT, 256>, a, p, cluster, 256, 0, s)
-                          : launch_clusters(logits_sum_kernel<DT, kNarrow>, a, p, cluster, kNarrow, 0, s);
+    return threads == kWide ? launch_clusters(logits_sum_kernel<DT, kWide>, a, p, cluster, kWide, s)
+                          : launch_clusters(logits_sum_kernel<DT, kNarrow>, a, p, cluster, kNarrow, s);
 }
 
 // every row of the gradient starts at the same place of a 16-byte group as its logits do
@@ -1127,7 +1136,8 @@ int launch_logits(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, cuda
     const size_t esz = dtype_bytes(dtype);
     const uint64_t groups = a.vocab / (16 / esz);
     const bool fits = MODE != kModePolicy || groups <= (uint64_t)kMostCluster * kWide * kMostHeld;
-    if ((MODE == kModePolicy && !alike(a, esz)) || !fits || groups < 64 || a.rows > 0x7FFFFFFFull / kMostCluster) return launch_rows<MODE>(a, p, dtype, nullptr, nullptr, s);
+    if ((MODE == kModePolicy && !alike(a, esz)) || !fits || groups < 64 || a.rows > 0x7FFFFFFFull / kMostCluster)
+        return launch_rows<MODE>(a, p, dtype, nullptr, nullptr, s);
     if (dtype == RLCU_F16) return launch_logits_dt<RLCU_F16, MODE>(a, p, sms, groups, s);
     if (dtype == RLCU_BF16) return launch_logits_dt<RLCU_BF16, MODE>(a, p, sms, groups, s);
     return launch_logits_dt<RLCU_F32, MODE>(a, p, sms, groups, s);
@@ -1149,7 +1159,7 @@ int launch_grad(const LogitsArgs& a, uint32_t dtype, const float* lse, const flo
 int launch_policy(const float* logp, uint64_t tokens, const int32_t* targets, uint32_t vocab, const PolicyArgs& p,
                   float* coef, rlcu_policy_stat* stat, uint32_t flags, bool behind, cudaStream_t s) {
     cudaLaunchAttribute attr[2];
-    cudaLaunchConfig_t cfg = cluster_launch(attr, tokens <= kVectorThreads ? 1 : tokens <= 4 * kVectorThreads ? 4 : 8, kVectorThreads, 0, s);
+    cudaLaunchConfig_t cfg = cluster_launch(attr, tokens <= kVectorThreads ? 1 : tokens <= 4 * kVectorThreads ? 4 : 8, kVectorThreads, s);
     if (behind) {
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -1236,7 +1246,7 @@ extern "C" int rlcu_preference_loss(const float* logp, uint64_t tokens, const fl
     while (cluster < kMostCluster && (uint64_t)cluster < pairs && tokens > (uint64_t)cluster * 4096) cluster *= 2;
     if (cluster > 8) RLCU_CUDA(cudaFuncSetAttribute(preference_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = cluster_launch(attr, cluster, kVectorThreads, 0, (cudaStream_t)stream);
+    cudaLaunchConfig_t cfg = cluster_launch(attr, cluster, kVectorThreads, (cudaStream_t)stream);
     RLCU_CUDA(cudaLaunchKernelEx(&cfg, preference_kernel, a));
     return RLCU_OK;
 }
