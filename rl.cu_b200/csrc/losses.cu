@@ -162,9 +162,8 @@ struct Online {
         e = most;
     }
     __device__ __forceinline__ void merge_warp() {
-        float most = e;
-#pragma unroll
-        for (int mask = 16; mask >= 1; mask >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, mask));
+        float most;
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(most) : "f"(e));      // (sm_100a; NaN is passed over)
         s *= exp2_fast(e - most);
         e = most;
 #pragma unroll
@@ -496,7 +495,7 @@ struct RowFeed {
 // and keeps it in registers between the sum and the gradient: the logits are read once, the gradient is written once.
 // Several clusters share an SM (four CTAs of 256 threads with up to ten groups each: 160 KB of its registers), so that
 // one row's loads and stores run under another's arithmetic.
-// Measured (B200, a tenth of the rows without part): 4096 x 151936 bf16 464 us, 0.78 of the copy rate (6.55 TB/s) for the
+// Measured (B200, a tenth of the rows without part): 4096 x 151936 bf16 457 us, 0.79 of the copy rate (6.55 TB/s) for the
 // bytes it cannot do without; 1000 x 151936 f32 229 us, 0.81.  A row takes a CTA about 14,500 cycles: 3,500 until its loads
 // are there, 3,000 for the sum, 3,000 to 4,500 to exchange it, 1,100 for the row's factors, 2,000 for the gradient; with
 // four CTAs per SM the special-function units and the issue slots are each a little over half busy.  The same kernel

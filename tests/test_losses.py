@@ -116,7 +116,7 @@ def test_oracle_policy_gradient_is_autograds(kl_kind, dual):
     loss = (w * (0.1 * k - best)).sum()
     loss.backward()
     l, kk, coef, _ = Q.policy(logp.detach(), old, ref, a, w, torch.ones(n, dtype=torch.bool), 0.2, 0.28, dual, 0.1, kl_kind)
-    assert abs(float((w * (l + 0.1 * kk)).sum()) - float(loss)) < 1e-12 * n
+    assert abs(float((w * (l + 0.1 * kk)).sum().detach()) - float(loss.detach())) < 1e-12 * n
     _, _, p, takes = Q.logprob(z.detach(), y)
     assert (Q.logits_grad(p, y, takes, coef) - z.grad).abs().max() < 1e-12
 
@@ -145,3 +145,19 @@ def test_oracle_preference_gradient_is_autograds(kind, mean, smoothing):
     (total / 3).backward()
     loss, _, _, coef, _ = Q.preference(logp.detach(), ref, mask, offsets, 3, 0.3, 0.05, smoothing, kind, mean)
     assert abs(loss - float(total) / 3) < 1e-12 and (coef - logp.grad).abs().max() < 1e-12
+
+
+def test_headers_are_plain_c(tmp_path):
+    """The three headers compile as C with nothing but each other."""
+    import os
+    import shutil
+    import subprocess
+    if shutil.which("gcc") is None:
+        pytest.skip("gcc not available")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "headers.c"
+    src.write_text("#include \"rlcu_act8.h\"\n#include \"rlcu_losses.h\"\n#include \"rlcu_adamw.h\"\n"
+                   "typedef char a[sizeof(rlcu_policy_stat) == 32 && sizeof(rlcu_preference_stat) == 32 ? 1 : -1];\n"
+                   "int main(void) { return RLCU_ACT8_BLOCK == 128 ? 0 : 1; }\n")
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Wextra", "-Werror", "-pedantic", "-I", os.path.join(root, "include"), "-c", str(src),
+                    "-o", str(tmp_path / "headers.o")], check=True)

@@ -636,3 +636,37 @@ def test_policy_loss_reads_what_ran_before_it(pkg):
         torch.cuda.synchronize()
         results.append((z, logp, coef, stat, stat2))
     assert all(torch.equal(p, q) for p, q in zip(*results))
+
+
+def test_logprob_without_lse(pkg):
+    z, y = gaussian(20, 5001, "bf16", 8).cuda(), targets_of(20, 5001, 8).cuda()
+    a, b, lse = torch.empty(20, device="cuda"), torch.empty(20, device="cuda"), torch.empty(20, device="cuda")
+    pkg.token_logprob(z.data_ptr(), pkg.BF16, 20, 5001, y.data_ptr(), a.data_ptr())
+    pkg.token_logprob(z.data_ptr(), pkg.BF16, 20, 5001, y.data_ptr(), b.data_ptr(), lse.data_ptr())
+    torch.cuda.synchronize()
+    assert torch.equal(a, b)
+
+
+def test_policy_loss_in_chunks_accumulates(pkg):
+    """The fused call on chunks of a batch, as the output projection hands them over: gradients and log-probabilities are those
+    of the whole, bit for bit where the chunks take the same kernel, and the record adds up."""
+    rows, vocab, chunk = 512, 6000, 128
+    z, y = gaussian(rows, vocab, "f16", 9).cuda(), targets_of(rows, vocab, 9).cuda()
+    g = torch.Generator().manual_seed(9)
+    a, w = torch.randn(rows, generator=g).cuda(), (torch.rand(rows, generator=g) / rows).cuda()
+    hp = pkg.policy_hparams()
+    out = []
+    for step in (rows, chunk):
+        logp, grad, stat = torch.empty(rows, device="cuda"), torch.empty_like(z), torch.zeros(8, dtype=torch.int32, device="cuda")
+        for r in range(0, rows, step):
+            pkg.policy_loss(z[r:].data_ptr(), pkg.F16, step, vocab, y[r:].data_ptr(), a[r:].data_ptr(), w[r:].data_ptr(), hp, logp[r:].data_ptr(),
+                            grad[r:].data_ptr(), stat.data_ptr(), flags=pkg.LOSS_ACCUMULATE if r else 0)
+        torch.cuda.synchronize()
+        out.append((logp, grad, stat_of(pkg.PolicyStat, stat)))
+    e = Q.logprob_error(z.cpu(), y.cpu(), 1.0) + 2.0 ** -19
+    close(out[1][0].cpu(), out[0][0].cpu(), 2 * e, "logp")
+    x, s = out[0][2], out[1][2]
+    assert (x.tokens, x.clipped) == (s.tokens, s.clipped)
+    size = float((w * a.abs()).sum())
+    assert abs(x.loss - s.loss) <= size * 8 * 2.0 ** -24 + float((w.cpu() * a.cpu().abs() * 2 * e).sum())
+    assert abs(x.weight - s.weight) <= x.weight * 8 * 2.0 ** -24
