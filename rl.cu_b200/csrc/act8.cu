@@ -788,10 +788,11 @@ norm_grad_vec_kernel(NormArgs a) {
     if (a.dweight) add_parts_in_cluster(a);
 }
 
-// Rows that start anywhere: thread t of the TPR that have a row takes columns t, t + TPR, ..., kColumns at most, one
-// element per access (a warp's 32 are side by side).  Bound by its many accesses: 16384 x 4001 bf16 111 us forward, 340 us
-// with gradient (rows read twice, one CTA each: 182 and 1067 us).
-constexpr int kColumns = 8;
+// Rows that start anywhere: thread t of the TPR that have a row takes columns t, t + TPR, ..., K at most, one element per
+// access (a warp's 32 are side by side); the next row's are on their way.  Bound by its many accesses.  TPR and K by the
+// width, as measured (bf16; eight columns of every thread beside it): gradient, 20000 x 300 38 us (89), 20000 x 1001 70 (96),
+// 16384 x 4001 264 (289), 9000 x 6001 364 (458, less room per SM); forward, 20000 x 300 23 (31), 9000 x 1501 38 (55).
+// There eight are better where four would be added up over more warps: 20000 x 1001 37 (39 of four), 16384 x 4001 103 (191).
 
 // one code without its scale
 __device__ __forceinline__ float code_value(uint8_t code) {
@@ -801,15 +802,15 @@ __device__ __forceinline__ float code_value(uint8_t code) {
 }
 
 // A thread's columns of one row: codes, and the scales of the blocks they lie in.
-template <int TPR>
+template <int TPR, int K>
 struct Columns {
-    uint8_t code[kColumns], byte[kColumns];
+    uint8_t code[K], byte[K];
 
-    __device__ __forceinline__ Columns(const NormArgs& a, uint32_t row, uint32_t lane) {
+    __device__ __forceinline__ void load(const NormArgs& a, uint32_t row, uint32_t lane) {
         const uint8_t* c = a.codes + row * a.code_stride + lane;
         const uint8_t* s = a.scales + (uint64_t)row * a.blocks + lane / kBlock;
 #pragma unroll
-        for (int k = 0; k < kColumns; k++) {
+        for (int k = 0; k < K; k++) {
             const bool in = lane + k * TPR < a.cols;
             code[k] = in ? c[k * TPR] : 0;
             byte[k] = in ? s[k * TPR / (int)kBlock] : 0;          // TPR = 32: a warp's columns lie in one block
@@ -818,22 +819,25 @@ struct Columns {
     __device__ __forceinline__ float scale(int k) const { return pow2((int)byte[k] - 127); }
 };
 
-template <uint32_t DT, int TPR, int THREADS>
+template <uint32_t DT, int TPR, int THREADS, int K>
 __global__ void __launch_bounds__(THREADS)
 norm_col_kernel(NormArgs a, uint32_t rows_per_cta) {
     using E = Elem<DT>;
     __shared__ RowSum<TPR, THREADS> sum;
     const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows;
     const uint32_t first = blockIdx.x * rows_per_cta + threadIdx.x / TPR, last = min(rows, (blockIdx.x + 1) * rows_per_cta);
-    float w[kColumns];
+    float w[K];
 #pragma unroll
-    for (int k = 0; k < kColumns; k++) w[k] = lane + k * TPR < a.cols ? weight_at(a, lane + k * TPR) : 0.0f;
+    for (int k = 0; k < K; k++) w[k] = lane + k * TPR < a.cols ? weight_at(a, lane + k * TPR) : 0.0f;
+    Columns<TPR, K> next;
+    if (first < last) next.load(a, first, lane);
     uint32_t step = 0;
     for (uint32_t row = first; row < last; row += THREADS / TPR, step++) {
-        const Columns<TPR> x(a, row, lane);
-        float c[kColumns], sq = 0.0f;
+        const Columns<TPR, K> x = next;
+        if (row + THREADS / TPR < last) next.load(a, row + THREADS / TPR, lane);
+        float c[K], sq = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kColumns; k++) {
+        for (int k = 0; k < K; k++) {
             c[k] = code_value(x.code[k]);
             const float v = c[k] * x.scale(k);
             sq = fmaf(v, v, sq);
@@ -842,70 +846,85 @@ norm_col_kernel(NormArgs a, uint32_t rows_per_cta) {
         if (a.rstd && lane == 0) a.rstd[row] = rstd;
         typename E::T* out = static_cast<typename E::T*>(a.out) + row * a.out_stride + lane;
 #pragma unroll
-        for (int k = 0; k < kColumns; k++)
+        for (int k = 0; k < K; k++)
             if (lane + k * TPR < a.cols) out[k * TPR] = E::down(c[k] * (x.scale(k) * rstd) * w[k]);
     }
 }
 
-template <uint32_t DT, int TPR, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS <= 256 ? 3 : THREADS <= 512 ? 2 : 1)
-norm_grad_col_kernel(NormArgs a) {
-    using E = Elem<DT>;
-    using T = typename E::T;
-    __shared__ RowSum<TPR, THREADS> sum;
-    const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows, at_once = THREADS / TPR, jump = gridDim.x * at_once;
-    float w[kColumns], dw[kColumns];
-#pragma unroll
-    for (int k = 0; k < kColumns; k++) {
-        w[k] = lane + k * TPR < a.cols ? weight_at(a, lane + k * TPR) : 0.0f;
-        dw[k] = 0.0f;
-    }
-    uint32_t step = 0;
-    for (uint32_t row = blockIdx.x * at_once + threadIdx.x / TPR; row < rows; row += jump, step++) {
+template <uint32_t DT, int TPR, int K>
+struct GradColumns {
+    Columns<TPR, K> x;
+    typename Elem<DT>::T d[K], r[K];
+
+    __device__ __forceinline__ void load(const NormArgs& a, uint32_t row, uint32_t lane) {
+        using T = typename Elem<DT>::T;
         const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride + lane;
         const T* dres = static_cast<const T*>(a.dres) + row * a.dres_stride + lane;
-        T* out = static_cast<T*>(a.out) + row * a.out_stride + lane;
-        const Columns<TPR> x(a, row, lane);
-        T d[kColumns], r[kColumns];
+        x.load(a, row, lane);
 #pragma unroll
-        for (int k = 0; k < kColumns; k++) {
+        for (int k = 0; k < K; k++) {
             const bool in = lane + k * TPR < a.cols;
             d[k] = in ? dy[k * TPR] : (T)0;
             r[k] = in && a.dres ? dres[k * TPR] : (T)0;
         }
+    }
+};
+
+template <uint32_t DT, int TPR, int THREADS, int K>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+norm_grad_col_kernel(NormArgs a) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    constexpr bool kAhead = K <= 4;            // two rows of eight columns would spill
+    __shared__ RowSum<TPR, THREADS> sum;
+    const uint32_t lane = threadIdx.x % TPR, rows = (uint32_t)a.rows, at_once = THREADS / TPR, jump = gridDim.x * at_once;
+    float w[K], dw[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        w[k] = lane + k * TPR < a.cols ? weight_at(a, lane + k * TPR) : 0.0f;
+        dw[k] = 0.0f;
+    }
+    uint32_t step = 0, row = blockIdx.x * at_once + threadIdx.x / TPR;
+    GradColumns<DT, TPR, K> next;
+    if (kAhead && row < rows) next.load(a, row, lane);
+    for (; row < rows; row += jump, step++) {
+        if (!kAhead) next.load(a, row, lane);
+        const GradColumns<DT, TPR, K> now = next;
+        if (kAhead && row + jump < rows) next.load(a, row + jump, lane);
+        T* out = static_cast<T*>(a.out) + row * a.out_stride + lane;
         float sq = 0.0f, dot = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kColumns; k++) {
-            const float v = code_value(x.code[k]) * x.scale(k);
+        for (int k = 0; k < K; k++) {
+            const float v = code_value(now.x.code[k]) * now.x.scale(k);
             sq = fmaf(v, v, sq);
-            dot = fmaf(E::up(d[k]) * w[k], v, dot);
+            dot = fmaf(E::up(now.d[k]) * w[k], v, dot);
         }
         const float2 sums = sum(sq, dot, step);
         const float rstd = 1.0f / sqrtf(sums.x / (float)a.cols + a.eps);
         const float pull = sums.y / (float)a.cols * rstd * rstd;
 #pragma unroll
-        for (int k = 0; k < kColumns; k++) {
+        for (int k = 0; k < K; k++) {
             if (lane + k * TPR >= a.cols) continue;
-            const float c = code_value(x.code[k]), s = x.scale(k), dk = E::up(d[k]);
+            const float c = code_value(now.x.code[k]), s = now.x.scale(k), dk = E::up(now.d[k]);
             dw[k] = fmaf(dk, c * (s * rstd), dw[k]);
-            out[k * TPR] = E::down(fmaf(rstd, fmaf(-c, s * pull, dk * w[k]), a.dres ? E::up(r[k]) : 0.0f));
+            out[k * TPR] = E::down(fmaf(rstd, fmaf(-c, s * pull, dk * w[k]), a.dres ? E::up(now.r[k]) : 0.0f));
         }
     }
     if (!a.partial) return;
     float* part = a.partial + (uint64_t)blockIdx.x * a.cols;
     if constexpr (TPR < THREADS) {
         // the CTA's groups have the same columns: the first to the last, in turn
-        __shared__ float shared[TPR * kColumns];
+        __shared__ float shared[TPR * K];
         for (int turn = 0; turn < (int)at_once; turn++) {
             if (threadIdx.x / TPR == turn)
 #pragma unroll
-                for (int k = 0; k < kColumns; k++) shared[lane + k * TPR] = turn ? shared[lane + k * TPR] + dw[k] : dw[k];
+                for (int k = 0; k < K; k++) shared[lane + k * TPR] = turn ? shared[lane + k * TPR] + dw[k] : dw[k];
             __syncthreads();
         }
         for (uint32_t j = threadIdx.x; j < a.cols; j += THREADS) part[j] = shared[j];
     } else {
 #pragma unroll
-        for (int k = 0; k < kColumns; k++)
+        for (int k = 0; k < K; k++)
             if (lane + k * TPR < a.cols) part[lane + k * TPR] = dw[k];
     }
     if (a.dweight) add_parts_in_cluster(a);
@@ -938,10 +957,11 @@ norm_weight_kernel(const float* partial, uint32_t parts, uint32_t cols, float* d
 // host side
 // ---------------------------------------------------------------------------
 
-// CTAs the rows of a gradient are dealt to, at most: what the registers of 148 SMs hold of 256 threads each
-constexpr uint64_t kMostParts = 2 * 148;
-
-uint64_t norm_parts(uint64_t rows) { return rows < kMostParts ? rows : kMostParts; }
+// CTAs the rows of a gradient are dealt to, at most: what the registers of 148 SMs hold of the kernels for that width
+uint64_t norm_parts(uint64_t rows, uint64_t cols) {
+    const uint64_t most = 148 * (cols <= 1024 ? 4 : 2);
+    return rows < most ? rows : most;
+}
 
 int check_matrix(const char* what, const void* p, uint32_t dtype, uint64_t rows, uint64_t cols, uint64_t& stride) {
     if (!dtype_known(dtype)) return set_error(RLCU_ERR_INVALID, "unknown dtype %u", dtype);
@@ -992,11 +1012,11 @@ int launch_norm_vec(const NormArgs& a, cudaStream_t s) {
     return RLCU_OK;
 }
 
-template <uint32_t DT, int TPR, int THREADS>
+template <uint32_t DT, int TPR, int THREADS, int K>
 int launch_norm_col(const NormArgs& a, cudaStream_t s) {
     uint32_t per = THREADS / TPR * 8;
     while (per > THREADS / TPR && a.rows / per < 148 * 2048 / THREADS) per /= 2;
-    norm_col_kernel<DT, TPR, THREADS><<<(unsigned)((a.rows + per - 1) / per), THREADS, 0, s>>>(a, per);
+    norm_col_kernel<DT, TPR, THREADS, K><<<(unsigned)((a.rows + per - 1) / per), THREADS, 0, s>>>(a, per);
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
 }
@@ -1010,10 +1030,12 @@ int launch_norm(const NormArgs& a, bool vec, cudaStream_t s) {
         if (a.cols <= 4096) return launch_norm_vec<DT, 256, 256>(a, s);
         return launch_norm_vec<DT, 512, 512>(a, s);
     }
-    if (a.cols <= 32 * kColumns) return launch_norm_col<DT, 32, 256>(a, s);
-    if (a.cols <= 128 * kColumns) return launch_norm_col<DT, 128, 256>(a, s);
-    if (a.cols <= 512 * kColumns) return launch_norm_col<DT, 512, 512>(a, s);
-    if (a.cols <= 1024 * kColumns) return launch_norm_col<DT, 1024, 1024>(a, s);
+    if (a.cols <= 128) return launch_norm_col<DT, 32, 256, 4>(a, s);
+    if (a.cols <= 512) return launch_norm_col<DT, 128, 256, 4>(a, s);
+    if (a.cols <= 1024) return launch_norm_col<DT, 128, 256, 8>(a, s);
+    if (a.cols <= 2048) return launch_norm_col<DT, 512, 512, 4>(a, s);
+    if (a.cols <= 4096) return launch_norm_col<DT, 512, 512, 8>(a, s);
+    if (a.cols <= kMostVecCols) return launch_norm_col<DT, 1024, 1024, 8>(a, s);
     int grid = 0;
     if (const int rc = grid_for(a.rows, 8, &grid)) return rc;
     norm_kernel<DT><<<grid, kAct8Threads, 0, s>>>(a);
@@ -1027,8 +1049,8 @@ int launch_norm(const NormArgs& a, bool vec, cudaStream_t s) {
 constexpr uint64_t kClusterSteps = 96;
 
 template <typename Kernel>
-int launch_grad_kernel(Kernel kernel, NormArgs a, int threads, uint64_t steps, float* dweight, uint32_t flags, int* parts, cudaStream_t s) {
-    *parts = (int)norm_parts(steps);
+int launch_grad_kernel(Kernel kernel, NormArgs a, int threads, uint64_t steps, uint64_t most, float* dweight, uint32_t flags, int* parts, cudaStream_t s) {
+    *parts = (int)(steps < most ? steps : most);
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = {};
     if (dweight && steps * threads <= kClusterSteps * 256) {
@@ -1055,13 +1077,13 @@ int launch_grad_kernel(Kernel kernel, NormArgs a, int threads, uint64_t steps, f
 template <uint32_t DT, int TPR, int THREADS>
 int launch_norm_grad_vec(const NormArgs& a, float* dweight, uint32_t flags, int* parts, cudaStream_t s) {
     constexpr uint64_t kAtOnce = THREADS / TPR;
-    return launch_grad_kernel(norm_grad_vec_kernel<DT, TPR, THREADS>, a, THREADS, (a.rows + kAtOnce - 1) / kAtOnce, dweight, flags, parts, s);
+    return launch_grad_kernel(norm_grad_vec_kernel<DT, TPR, THREADS>, a, THREADS, (a.rows + kAtOnce - 1) / kAtOnce, 148 * (THREADS <= 256 ? 2 : 1), dweight, flags, parts, s);
 }
 
-template <uint32_t DT, int TPR, int THREADS>
+template <uint32_t DT, int TPR, int THREADS, int K>
 int launch_norm_grad_col(const NormArgs& a, float* dweight, uint32_t flags, int* parts, cudaStream_t s) {
     constexpr uint64_t kAtOnce = THREADS / TPR;
-    return launch_grad_kernel(norm_grad_col_kernel<DT, TPR, THREADS>, a, THREADS, (a.rows + kAtOnce - 1) / kAtOnce, dweight, flags, parts, s);
+    return launch_grad_kernel(norm_grad_col_kernel<DT, TPR, THREADS, K>, a, THREADS, (a.rows + kAtOnce - 1) / kAtOnce, 148 * 1024 / THREADS, dweight, flags, parts, s);
 }
 
 template <uint32_t DT>
@@ -1073,11 +1095,13 @@ int launch_norm_grad(const NormArgs& a, bool vec, float* dweight, uint32_t flags
         if (a.cols <= 4096) return launch_norm_grad_vec<DT, 256, 256>(a, dweight, flags, parts, s);
         return launch_norm_grad_vec<DT, 512, 512>(a, dweight, flags, parts, s);
     }
-    if (a.cols <= 32 * kColumns) return launch_norm_grad_col<DT, 32, 256>(a, dweight, flags, parts, s);
-    if (a.cols <= 128 * kColumns) return launch_norm_grad_col<DT, 128, 256>(a, dweight, flags, parts, s);
-    if (a.cols <= 512 * kColumns) return launch_norm_grad_col<DT, 512, 512>(a, dweight, flags, parts, s);
-    if (a.cols <= 1024 * kColumns) return launch_norm_grad_col<DT, 1024, 1024>(a, dweight, flags, parts, s);
-    *parts = (int)norm_parts(a.rows);
+    if (a.cols <= 128) return launch_norm_grad_col<DT, 32, 256, 4>(a, dweight, flags, parts, s);
+    if (a.cols <= 512) return launch_norm_grad_col<DT, 128, 256, 4>(a, dweight, flags, parts, s);
+    if (a.cols <= 1024) return launch_norm_grad_col<DT, 256, 256, 4>(a, dweight, flags, parts, s);
+    if (a.cols <= 2048) return launch_norm_grad_col<DT, 512, 512, 4>(a, dweight, flags, parts, s);
+    if (a.cols <= 4096) return launch_norm_grad_col<DT, 1024, 1024, 4>(a, dweight, flags, parts, s);
+    if (a.cols <= kMostVecCols) return launch_norm_grad_col<DT, 1024, 1024, 8>(a, dweight, flags, parts, s);
+    *parts = (int)norm_parts(a.rows, a.cols);
     norm_grad_kernel<DT><<<*parts, kAct8Threads, 0, s>>>(a);
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
@@ -1090,7 +1114,7 @@ using namespace rlcu;
 
 extern "C" uint64_t rlcu_act8_blocks(uint64_t cols) { return (cols + kBlock - 1) / kBlock; }
 
-extern "C" uint64_t rlcu_act8_rmsnorm_grad_workspace(uint64_t rows, uint64_t cols) { return norm_parts(rows) * cols * sizeof(float); }
+extern "C" uint64_t rlcu_act8_rmsnorm_grad_workspace(uint64_t rows, uint64_t cols) { return norm_parts(rows, cols) * cols * sizeof(float); }
 
 extern "C" int rlcu_act8_store(const void* x, uint32_t dtype, uint64_t rows, uint64_t cols, uint64_t x_stride,
                                uint8_t* codes, uint64_t code_stride, uint8_t* scales, void* stream) {

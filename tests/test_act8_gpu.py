@@ -225,6 +225,14 @@ def test_norm_many_rows(pkg, rows, cols):
     check_norm_grad(pkg, rows, cols, "bf16", rows)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(5000, 77), (1300, 500), (700, 513), (650, 1001), (400, 1501), (310, 4001), (300, 6001), (160, 8191)])
+def test_norm_many_rows_that_start_anywhere(pkg, rows, cols, dtype):
+    """More rows than CTAs, at each width that has threads of its own: the row ahead, and the sums over a CTA's rows."""
+    check_norm(pkg, rows, cols, dtype, rows)
+    check_norm_grad(pkg, rows, cols, dtype, rows, residual=dtype == "bf16")
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("cpad,coffset,pad,offset,dpad,doffset", [(0, 0, 3, 1, 0, 0), (1, 1, 0, 0, 0, 0), (16, 0, 8, 0, 16, 0), (8, 8, 8, 8, 8, 8), (0, 0, 0, 0, 1, 3), (0, 4, 4, 4, 4, 4)])
 def test_norm_strides_and_offsets(pkg, dtype, cpad, coffset, pad, offset, dpad, doffset):
