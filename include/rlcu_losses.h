@@ -92,7 +92,8 @@ int rlcu_policy_loss_logp(const float* logp, uint64_t tokens, const float* old_l
                           const float* advantage, const float* weight, const rlcu_policy_hparams* hp /* host */,
                           float* coef, rlcu_policy_stat* stat, uint32_t flags, void* stream);
 /* The loss of a block of logits and its gradient in one call: the logits are read from memory once and the
- * gradient is written once.  `logp` receives the log-probabilities.  `grad` may be NULL: the loss alone. */
+ * gradient is written once.  `logp` receives the log-probabilities and is a buffer of its own, not that of old_logp.
+ * `grad` may be NULL: the loss alone. */
 int rlcu_policy_loss(const void* logits, uint32_t dtype, uint64_t rows, uint64_t vocab, uint64_t row_stride,
                      float inv_temperature, const int32_t* targets, const float* old_logp, const float* ref_logp,
                      const float* advantage, const float* weight, const rlcu_policy_hparams* hp /* host */,
@@ -132,7 +133,7 @@ typedef struct rlcu_preference_stat {
  *   ref_logp    : NULL: without a reference
  *   mask        : one byte per token, 0 takes no part (NULL: all do); what a masked place holds does not matter
  *   pair_weight : NULL: 1/pairs each
- *   coef        : dloss/dlogp, 0 for masked tokens and for tokens of no sequence; may be NULL
+ *   coef        : dloss/dlogp, 0 for masked tokens and for tokens of no sequence; may be NULL, and may be the buffer of logp
  *   rewards     : beta * s of each sequence; may be NULL
  * A sequence without tokens has s = 0. */
 int rlcu_preference_loss(const float* logp, uint64_t tokens, const float* ref_logp, const uint8_t* mask,

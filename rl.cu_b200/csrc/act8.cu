@@ -1180,6 +1180,7 @@ extern "C" int rlcu_act8_rmsnorm(const uint8_t* codes, uint64_t code_stride, con
     if (const int rc = check_matrix("y", y, dtype, rows, cols, y_stride)) return rc;
     if (const int rc = check_matrix("weight", weight, weight_dtype, 1, cols, one)) return rc;
     if (!(eps >= 0.0f) || std::isinf(eps)) return set_error(RLCU_ERR_INVALID, "eps must be finite and not negative");
+    if (!words_aligned({rstd})) return set_error(RLCU_ERR_INVALID, "rstd: not aligned to its element size");
     if (!rows || !cols) return RLCU_OK;
     if (overlap(span_of(y, rows, cols, y_stride, dtype_bytes(dtype)), span_of(codes, rows, cols, code_stride, 1)))
         return set_error(RLCU_ERR_INVALID, "y and codes overlap");
@@ -1206,6 +1207,7 @@ extern "C" int rlcu_act8_rmsnorm_grad(const uint8_t* codes, uint64_t code_stride
         if (const int rc = check_matrix("dresidual", dresidual, dtype, rows, cols, dresidual_stride)) return rc;
     if (const int rc = check_matrix("weight", weight, weight_dtype, 1, cols, one)) return rc;
     if (!(eps >= 0.0f) || std::isinf(eps)) return set_error(RLCU_ERR_INVALID, "eps must be finite and not negative");
+    if (!words_aligned({dweight})) return set_error(RLCU_ERR_INVALID, "dweight: not aligned to its element size");
     if (flags & ~(uint32_t)RLCU_ACT8_ACCUMULATE) return set_error(RLCU_ERR_INVALID, "unknown flags");
     const size_t esz = dtype_bytes(dtype);
     if (!same_or_apart(dx, dx_stride, dy, dy_stride, rows, cols, esz) ||

@@ -1047,6 +1047,15 @@ int check_policy(const rlcu_policy_hparams* hp, const float* ref_logp, const flo
     return RLCU_OK;
 }
 
+const char* const kUnaligned = "a vector of 4-byte values is not aligned to them";
+
+// `out` (n FP32 values) shares none of its bytes with the inputs, or (with `same`) all of them
+bool out_apart(const float* out, uint64_t n, std::initializer_list<const float*> inputs, bool same) {
+    for (const float* in : inputs)
+        if (out && in && !(same && in == out) && overlap(span_of(out, 1, n, n, 4), span_of(in, 1, n, n, 4))) return false;
+    return true;
+}
+
 int sm_count(int* out) {
     int dev = 0;
     RLCU_CUDA(cudaGetDevice(&dev));
@@ -1177,6 +1186,7 @@ extern "C" int rlcu_token_logprob(const void* logits, uint32_t dtype, uint64_t r
                                   float inv_temperature, const int32_t* targets, float* logp, float* lse, void* stream) {
     if (const int rc = check_logits(logits, dtype, rows, vocab, row_stride, inv_temperature, targets)) return rc;
     if (rows && !logp) return set_error(RLCU_ERR_INVALID, "null logp");
+    if (!words_aligned({targets, logp, lse})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
     if (!rows) return RLCU_OK;
     LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, logp, lse, nullptr, 0, nullptr};
     return launch_logits<kModeLogprob>(a, PolicyArgs{}, dtype, (cudaStream_t)stream);
@@ -1189,6 +1199,7 @@ extern "C" int rlcu_token_logprob_grad(const void* logits, uint32_t dtype, uint6
     if (const int rc = check_logits(logits, dtype, rows, vocab, row_stride, inv_temperature, targets)) return rc;
     if (const int rc = check_grad(logits, dtype, rows, vocab, row_stride, grad, grad_stride)) return rc;
     if (rows && (!lse || !coef)) return set_error(RLCU_ERR_INVALID, "null lse or coef");
+    if (!words_aligned({targets, lse, coef, scaler})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
     if (!rows) return RLCU_OK;
     LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, nullptr, nullptr, grad, grad_stride, scaler};
     return launch_grad(a, dtype, lse, coef, (cudaStream_t)stream);
@@ -1199,6 +1210,9 @@ extern "C" int rlcu_policy_loss_logp(const float* logp, uint64_t tokens, const f
                                      float* coef, rlcu_policy_stat* stat, uint32_t flags, void* stream) {
     if (const int rc = check_policy(hp, ref_logp, advantage, weight, stat, tokens, flags)) return rc;
     if (tokens && !logp) return set_error(RLCU_ERR_INVALID, "null logp");
+    if (!words_aligned({logp, old_logp, ref_logp, advantage, weight, coef})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
+    if (!out_apart(coef, tokens, {logp, old_logp, ref_logp, advantage, weight}, true))
+        return set_error(RLCU_ERR_INVALID, "coef overlaps an input without being the same buffer");
     PolicyArgs p = {old_logp, ref_logp, advantage, weight, *hp};
     return launch_policy(logp, tokens, nullptr, 0, p, coef, stat, flags, false, (cudaStream_t)stream);
 }
@@ -1213,6 +1227,10 @@ extern "C" int rlcu_policy_loss(const void* logits, uint32_t dtype, uint64_t row
     if (grad)
         if (const int rc = check_grad(logits, dtype, rows, vocab, row_stride, grad, grad_stride)) return rc;
     if (rows && !logp) return set_error(RLCU_ERR_INVALID, "null logp");
+    if (!words_aligned({targets, old_logp, ref_logp, advantage, weight, logp, scaler})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
+    // logp is written before the record is formed from the inputs
+    if (!out_apart(logp, rows, {old_logp, ref_logp, advantage, weight}, false))
+        return set_error(RLCU_ERR_INVALID, "logp overlaps another input of the loss");
     LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, logp, nullptr, grad, grad_stride, scaler};
     PolicyArgs p = {old_logp, ref_logp, advantage, weight, *hp};
     if (rows) {
@@ -1239,6 +1257,8 @@ extern "C" int rlcu_preference_loss(const float* logp, uint64_t tokens, const fl
     if (!stat || reinterpret_cast<uintptr_t>(stat) % 16) return set_error(RLCU_ERR_INVALID, "the record must be given and 16-byte aligned");
     if (!offsets) return set_error(RLCU_ERR_INVALID, "null offsets");
     if (tokens && !logp) return set_error(RLCU_ERR_INVALID, "null logp");
+    if (!words_aligned({logp, ref_logp, offsets, pair_weight, coef, rewards})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
+    if (!out_apart(coef, tokens, {logp, ref_logp}, true)) return set_error(RLCU_ERR_INVALID, "coef overlaps an input without being the same buffer");
     PreferenceArgs a = {logp, ref_logp, mask, offsets, pair_weight, tokens, pairs, *hp, coef, rewards, stat, flags};
     // more CTAs than pairs would idle; below a few thousand tokens each, the cluster costs more than it saves
     int cluster = 1;

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "rlcu_adamw.h"
 
 namespace rlcu {
@@ -138,5 +140,12 @@ __host__ inline Span span_of(const void* p, uint64_t rows, uint64_t cols, uint64
     return {lo, rows && cols ? lo + ((rows - 1) * stride + cols) * esz : lo};
 }
 __host__ inline bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
+
+// vectors of 4-byte values (null: none), each aligned to them
+__host__ inline bool words_aligned(std::initializer_list<const void*> vectors) {
+    for (const void* p : vectors)
+        if (reinterpret_cast<uintptr_t>(p) % 4) return false;
+    return true;
+}
 
 }  // namespace rlcu

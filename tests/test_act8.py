@@ -74,6 +74,12 @@ def test_rmsnorm_refusals(pkg):
     refuse(pkg, "workspace", backward, n=pkg.act8_rmsnorm_grad_workspace(2, 8) - 1)
 
 
+def test_rmsnorm_refuses_vectors_that_are_not_aligned(pkg):
+    B, C, D = A + (1 << 16), A + (2 << 16), A + (3 << 16)
+    refuse(pkg, "rstd", pkg.act8_rmsnorm, A, B, 2, 8, C, pkg.F32, 1e-6, D, pkg.F16, A + 2)
+    refuse(pkg, "dweight", pkg.act8_rmsnorm_grad, A, B, 2, 8, C, pkg.F32, 1e-6, D, pkg.F16, D + 4096, C + 6, D + 8192, 1 << 20)
+
+
 def test_oracle_rounding_is_at_most_half_a_step():
     g = torch.Generator().manual_seed(0)
     x = torch.randn(40, 300, generator=g) * torch.exp(3 * torch.randn(40, 300, generator=g))

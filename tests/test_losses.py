@@ -161,3 +161,38 @@ def test_headers_are_plain_c(tmp_path):
                    "int main(void) { return RLCU_ACT8_BLOCK == 128 ? 0 : 1; }\n")
     subprocess.run(["gcc", "-std=c99", "-Wall", "-Wextra", "-Werror", "-pedantic", "-I", os.path.join(root, "include"), "-c", str(src),
                     "-o", str(tmp_path / "headers.o")], check=True)
+
+
+def test_vectors_that_overlap_or_are_not_aligned_are_refused(pkg):
+    """The log-probabilities a policy loss writes would be read as the old ones; odd addresses would fault the GPU."""
+    B, D = A + (1 << 16), A + (2 << 16)
+    ok = pkg.policy_hparams(0.2, 0.28, 3.0, 0.1)
+
+    def policy(old=B, ref=B, adv=B, w=B, logp=D, targets=B, scaler=None):
+        pkg.policy_loss(A, pkg.F16, 2, 8, targets, adv, w, ok, logp, None, A, old_logp=old, ref_logp=ref, scaler=scaler)
+
+    for name in ("old", "ref", "adv", "w"):
+        refuse(pkg, "overlap", policy, **{name: D})
+        refuse(pkg, "overlap", policy, **{name: D + 4})
+        refuse(pkg, "aligned", policy, **{name: B + 2})
+    for name in ("logp", "targets", "scaler"):
+        refuse(pkg, "aligned", policy, **{name: B + 1})
+
+    def vector(coef=D, logp=B, ref=B, adv=B, w=B, old=B):
+        pkg.policy_loss_logp(logp, 4, adv, w, ok, A, coef=coef, old_logp=old, ref_logp=ref)
+
+    for name in ("logp", "ref", "adv", "w", "old"):
+        refuse(pkg, "overlap", vector, **{name: D + 4})
+        refuse(pkg, "aligned", vector, **{name: B + 3})
+    refuse(pkg, "aligned", vector, coef=D + 2)
+
+    def preference(coef=D, logp=B, ref=B, offsets=B, weight=B, rewards=B):
+        pkg.preference_loss(logp, 4, offsets, 1, pkg.preference_hparams(0.1), A, coef=coef, rewards=rewards, ref_logp=ref, pair_weight=weight)
+
+    for name in ("logp", "ref"):
+        refuse(pkg, "overlap", preference, **{name: D - 8})
+    for name in ("coef", "logp", "ref", "offsets", "weight", "rewards"):
+        refuse(pkg, "aligned", preference, **{name: B + 2})
+    refuse(pkg, "aligned", pkg.token_logprob, A, pkg.F16, 1, 8, B + 2, B)
+    refuse(pkg, "aligned", pkg.token_logprob, A, pkg.F16, 1, 8, B, B + 2)
+    refuse(pkg, "aligned", pkg.token_logprob_grad, A, pkg.F16, 1, 8, B, B + 1, B, D)

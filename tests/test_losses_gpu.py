@@ -508,6 +508,24 @@ def test_preference_record_accumulates(pkg):
     assert (a.pairs, a.correct) == (b.pairs, b.correct) and abs(a.loss - b.loss) <= 3 * 2.0 ** -24 * 3
 
 
+@pytest.mark.parametrize("length", [3, 700])
+def test_preference_coefficients_in_the_buffer_of_the_log_probabilities(pkg, length):
+    """100 pairs of `length` tokens and 50 tokens of no sequence at either end: the same bits as in a buffer of their own."""
+    pairs = 100
+    offsets = torch.arange(2 * pairs + 1, dtype=torch.int32, device="cuda") * length + 50
+    tokens = 2 * pairs * length + 100
+    g = torch.Generator().manual_seed(length)
+    logp, ref = ((-torch.rand(tokens, generator=g) * 2).cuda() for _ in range(2))
+    results = []
+    for coef in (torch.full_like(logp, 7.0), logp):
+        stat, rewards = torch.zeros(8, dtype=torch.int32, device="cuda"), torch.zeros(2 * pairs, device="cuda")
+        pkg.preference_loss(logp.data_ptr(), tokens, offsets.data_ptr(), pairs, pkg.preference_hparams(0.1), stat.data_ptr(), coef.data_ptr(),
+                            rewards.data_ptr(), ref.data_ptr())
+        torch.cuda.synchronize()
+        results.append((coef, stat, rewards))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
 def test_preference_without_pairs(pkg):
     coef, stat = torch.full((9,), 7.0, device="cuda"), torch.full((8,), 7, dtype=torch.int32, device="cuda")
     lp, ob = torch.zeros(9, device="cuda"), torch.tensor([4], dtype=torch.int32, device="cuda")
