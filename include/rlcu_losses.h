@@ -14,9 +14,10 @@
  * The loss is that of logits * inv_temperature (in (0, 1e6]).  Values between the rows are neither read nor written.
  * A row takes part when its target is in [0, vocab) (and, in the policy loss, its weight is not zero); of a row
  * that takes no part the logits are not read, its log-probability is 0 and its gradient row is written as
- * zeros.  Logits of -inf are tokens of probability zero; a row with nothing but -inf has lse = logp = -inf and
- * probabilities of zero.  NaN and +inf make their row's results NaN, which the statistics pass
- * (rlcu_gradstat) then finds in the gradients.
+ * zeros.  Logits of -inf, and finite ones of -1e30 and below, are tokens of probability zero; a row with nothing else
+ * has lse = logp = -inf and probabilities of zero.  (Other masks, -1e9 or -1e20, are logits like any other: a row of
+ * nothing but one of them is uniform.)  NaN and +inf, and logits whose product with inv_temperature * log2 e is beyond
+ * FP32, make their row's results NaN, which the statistics pass (rlcu_gradstat) then finds in the gradients.
  *
  * Gradients are those of the loss times scaler->scale (the loss scale the statistics pass later divides out;
  * no scaler: 1), rounded once to the logits' type.  A gradient buffer may be the logits' own
@@ -39,7 +40,8 @@ int rlcu_token_logprob(const void* logits, uint32_t dtype, uint64_t rows, uint64
                        float inv_temperature, const int32_t* targets, float* logp, float* lse, void* stream);
 /* grad[t][j] = coef[t] * S * inv_temperature * ([j == targets[t]] - softmax_j), with coef[t] = dLoss/dlogp[t]
  * (coef = -1/tokens: the SFT loss of RL.cu) and S the loss scale; `lse` is what rlcu_token_logprob wrote for the
- * same logits.  A row with coef 0 takes no part. */
+ * same logits; a row whose |lse| is above 2^24, which FP32 holds too coarsely for a probability, has a gradient of NaN.
+ * A row with coef 0 takes no part. */
 int rlcu_token_logprob_grad(const void* logits, uint32_t dtype, uint64_t rows, uint64_t vocab, uint64_t row_stride,
                             float inv_temperature, const int32_t* targets, const float* lse, const float* coef,
                             const rlcu_scaler_state* scaler, void* grad, uint64_t grad_stride, void* stream);

@@ -1,7 +1,7 @@
 // Losses of a training step and the gradients they start the backward pass with (include/rlcu_losses.h).
 //
 // Mathematics, per row z of logits (t: inv_temperature, c = t * log2 e, y: target):
-//   E  = ceil(c * max z)            an integer, so that x_j = fma(z_j, c, -E) is rounded once
+//   E  = ceil(c * max z)            an integer, so that x_j = fma(z_j, c, -E) is rounded once (within 2^31: see Top)
 //   s  = sum 2^x_j                  one pass with a running E per thread, partial sums rescaled by powers of two
 //   logp = (x_y - log2 s) ln 2,     lse = (E + log2 s) ln 2
 //   dz_j = coef * S * t * ([j == y] - 2^x_j / s)
@@ -21,8 +21,7 @@ namespace {
 constexpr int kRowThreads = 512;
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// Where the running maximum starts: logits below it (-inf, and masks of a type's lowest value) add nothing,
-// and a row without any other has s = 0.
+// Logits of this and less (-inf, and masks of a type's lowest value) add nothing, and a row without any other has s = 0.
 constexpr float kNoLogit = -1e30f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -110,15 +109,19 @@ __device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& p, float log
 
 // Sum of 2^(c z - e) for an integer e that follows the largest c z: raised when terms pass 2^kSlack, so after a
 // thread's first group hardly ever.  The sum is a float: how far e lies below the largest term costs nothing.
+// It stays within 2^31: a larger one would be so coarse that the largest term itself is inf or 0 beside it.  Terms below
+// 2^-2^31 are zeros then, as they have to be beside any other, and a row without any other ends with s = 0; a term above
+// 2^2^31 makes s inf.  Such rows are looked at again (Top).
 constexpr float kSlack = 1099511627776.0f;            // 2^40
+constexpr float kFar = 2147483648.0f;                 // 2^31
 
 struct Online {
     float e;
     float s = 0.0f;
 
-    __device__ __forceinline__ explicit Online(float c) : e(ceilf(kNoLogit * c)) {}
+    __device__ __forceinline__ explicit Online(float c) : e(fmaxf(ceilf(kNoLogit * c), -kFar)) {}
     __device__ __forceinline__ void raise(float largest, float c) {
-        const float e_new = ceilf(largest * c);
+        const float e_new = ceilf(fminf(largest * c, kFar));
         if (e_new > e) {
             s *= exp2_fast(e - e_new);
             e = e_new;
@@ -169,12 +172,29 @@ struct Online {
 #pragma unroll
         for (int mask = 16; mask >= 1; mask >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, mask);
     }
-    // s in [1, 2), or 0, inf or NaN: x_y = c z_y - e is then no larger than its own logarithm
-    __device__ __forceinline__ void settle() {
-        if (s > 0.0f && s < INFINITY) {
-            const int k = (int)((__float_as_uint(s) >> 23) & 0xFFu) - 127;
-            s *= __uint_as_float((uint32_t)(127 - k) << 23);
-            e += (float)k;
+    // the sum says nothing of the row's largest logit
+    __device__ __forceinline__ bool says_nothing() const { return s == 0.0f || s == INFINITY; }
+};
+
+// The other look at a row: its largest logit m and how many there are of it.  With c m beyond 2^31 two different logits of
+// a type are 2^7 apart after the product with c, so that all but the largest add nothing to a float.
+struct Top {
+    float e = -INFINITY;           // m
+    float s = 0.0f;                // their number
+
+    __device__ __forceinline__ Top() {}
+    __device__ __forceinline__ explicit Top(float) {}
+    __device__ __forceinline__ void add(float z) { merge(z, z > kNoLogit ? 1.0f : 0.0f); }
+    __device__ __forceinline__ void merge(float e2, float s2) {
+        const float most = fmaxf(e, e2);
+        s = (e == most ? s : 0.0f) + (e2 == most ? s2 : 0.0f);
+        e = most;
+    }
+    __device__ __forceinline__ void merge_warp() {
+#pragma unroll
+        for (int mask = 16; mask >= 1; mask >>= 1) {
+            const float e2 = __shfl_xor_sync(0xFFFFFFFFu, e, mask), s2 = __shfl_xor_sync(0xFFFFFFFFu, s, mask);
+            merge(e2, s2);
         }
     }
 };
@@ -182,28 +202,64 @@ struct Online {
 // What one thread makes of a row's sum.
 struct RowAnswer {
     float logp, lse;
-    float e, inv;      // p_j = 2^(c z_j - e) * inv
+    float e, by, inv;  // p_j = 2^(by z_j - e) * inv
 };
 
-__device__ __forceinline__ RowAnswer row_answer(Online o, float z_y, float c) {
-    if (o.e == INFINITY) o.s = NAN;           // logits whose product with c is beyond FP32
-    o.settle();
-    const float l2 = log2f(o.s);
+// e is exact to 1 and more: rows of any usual logits
+constexpr float kExact = 8388608.0f;                  // 2^23
+
+// (o.s is neither 0 nor inf)
+template <bool NEAR>
+__device__ __forceinline__ RowAnswer row_answer(const Online& o, float z_y, float c) {
+    // s = s' 2^k with s' in [1, 2).  k goes into e, so that x_y = c z_y - e is no larger than its own logarithm, or, where
+    // that sum would be rounded, into x_y.
+    float e = o.e, t = o.s;
+    int k = 0;
+    if (o.s > 0.0f && o.s < INFINITY) {
+        k = (int)((__float_as_uint(o.s) >> 23) & 0xFFu) - 127;
+        t *= __uint_as_float((uint32_t)(127 - k) << 23);
+        if (NEAR || fabsf(e) < kExact) {
+            e += (float)k;
+            k = 0;
+        }
+    }
+    const float l2 = log2f(t), x_y = fmaf(z_y, c, -e);
     RowAnswer r;
-    r.logp = o.s == 0.0f ? -INFINITY : (fmaf(z_y, c, -o.e) - l2) * kLn2;      // 0: nothing but -inf in the row
-    r.lse = o.s == 0.0f ? -INFINITY : (o.e + l2) * kLn2;
-    r.e = o.e;
-    r.inv = o.s == 0.0f ? 0.0f : 1.0f / o.s;
+    r.by = c;
+    r.e = e;
+    r.logp = ((NEAR ? x_y : x_y - (float)k) - l2) * kLn2;
+    r.lse = ((NEAR ? e : e + (float)k) + l2) * kLn2;
+    r.inv = 1.0f / (NEAR || k == 0 ? t : o.s);
     return r;
 }
 
-// 16 bytes of gradient away from the target: kn 2^(c z - e)
+__device__ __forceinline__ RowAnswer row_answer(const Top& o, float z_y, float c, float inv_temperature) {
+    RowAnswer r;
+    if (o.s == 0.0f) {             // nothing but -inf in the row
+        r.logp = r.lse = -INFINITY;
+        r.e = INFINITY;
+        r.by = c;
+        r.inv = 0.0f;
+        return r;
+    }
+    // 2^31 <= |by m| < 2^32: exact, and any other logit is at least 2^7 away
+    const uint32_t exponent = (__float_as_uint(o.e) >> 23) & 0xFFu;
+    r.by = __uint_as_float((127u + 31u + 127u - exponent) << 23);
+    r.e = o.e * r.by;
+    r.inv = 1.0f / o.s;
+    r.logp = fmaf(z_y - o.e, inv_temperature, -logf(o.s));
+    r.lse = fmaf(o.e, inv_temperature, logf(o.s));
+    if (isinf(o.e * c)) r.logp = r.lse = r.inv = NAN;      // +inf, or logits whose product with c is beyond FP32
+    return r;
+}
+
+// 16 bytes of gradient away from the target: kn 2^(by z - e)
 template <uint32_t DT>
-__device__ __forceinline__ uint4 grad_group(uint4 v, float c, float e, float kn) {
+__device__ __forceinline__ uint4 grad_group(uint4 v, float by, float e, float kn) {
     using E = Elem<DT>;
     float f[E::kVec];
     E::unpack(v, f);
-    const F2 cc(c, c), ee(-e, -e), kk(kn, kn);
+    const F2 cc(by, by), ee(-e, -e), kk(kn, kn);
 #pragma unroll
     for (int i = 0; i < E::kVec; i += 2) {
         float x, y;
@@ -213,7 +269,46 @@ __device__ __forceinline__ uint4 grad_group(uint4 v, float c, float e, float kn)
     return E::pack(f);
 }
 
+// An FP32 log-sum-exp of more than this is off by up to a factor of e, and a probability taken from it is worth nothing:
+// the row's gradient is NaN.
+constexpr float kMostLse = 16777216.0f;               // 2^24
+__device__ __forceinline__ float usable(float lse) { return fabsf(lse) > kMostLse && lse != -INFINITY ? NAN : lse; }
+
+// Top of a row, by a warp (a call, so that its registers are not taken from those who hardly ever make it)
+template <uint32_t DT>
+__device__ __noinline__ Top top_by_warp(const typename Elem<DT>::T* x, uint32_t n) {
+    using E = Elem<DT>;
+    const RowCut cut = cut_row(x, n);
+    const uint32_t lane = threadIdx.x & 31;
+    Top o;
+#pragma unroll 4
+    for (uint32_t i = lane; i < cut.groups; i += 32) {
+        float f[E::kVec];
+        E::unpack(reinterpret_cast<const uint4*>(x + cut.head)[i], f);
+#pragma unroll
+        for (int q = 0; q < E::kVec; q++) o.add(f[q]);
+    }
+    if (lane < cut.head) o.add(E::up(x[lane]));
+    for (uint32_t i = cut.head + cut.groups * E::kVec + lane; i < n; i += 32) o.add(E::up(x[i]));
+    o.merge_warp();
+    return o;
+}
+
+// The sum over a CTA of up to 32 warps, in every thread.  Another call with the same parts needs a barrier before it.
+template <typename Sum>
+__device__ __forceinline__ Sum add_in_block(Sum o, float2* parts, float c) {
+    o.merge_warp();
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = make_float2(o.e, o.s);
+    __syncthreads();
+    Sum all(c);
+    if ((threadIdx.x & 31) < blockDim.x >> 5) all.merge(parts[threadIdx.x & 31].x, parts[threadIdx.x & 31].y);
+    all.merge_warp();
+    return all;
+}
+
 constexpr uint32_t kNoTarget = 0xFFFFFFFFu;
+// log-probability (a NaN that no arithmetic makes) of a row whose sum says nothing, until policy_kernel has looked again
+constexpr uint32_t kLookAgain = 0x7FC5EEDu << 4;
 enum { kModeLogprob = 0, kModeGrad = 1, kModePolicy = 2 };
 
 __device__ __forceinline__ bool row_takes_part(const LogitsArgs& a, const PolicyArgs& p, uint64_t row, int32_t y) {
@@ -241,7 +336,7 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
     using E = Elem<DT>;
     using T = typename E::T;
     __shared__ float2 warp_part[kRowThreads / 32];
-    __shared__ float4 answer;                         // e, -k / s, k (1 - p_y)
+    __shared__ float4 answer;                         // e, -k / s, k (1 - p_y), factor of z (policy kernel: 0 for a row to be looked at again)
     const float c = a.inv_temperature * kLog2E;
     const float S = a.scaler ? a.scaler->scale : 1.0f;
 
@@ -267,20 +362,17 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
             for (uint32_t i = threadIdx.x; i < cut.groups; i += kRowThreads) o.add<DT>(body[i], c);
             if (threadIdx.x < cut.head) o.add(E::up(x[threadIdx.x]), c);
             for (uint32_t i = tail + threadIdx.x; i < a.vocab; i += kRowThreads) o.add(E::up(x[i]), c);
-            o.merge_warp();
-            if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = make_float2(o.e, o.s);
-            __syncthreads();
+            o = add_in_block(o, warp_part, c);
             if (threadIdx.x < 32) {
-                Online all(c);
-                if (threadIdx.x < kRowThreads / 32) all.merge(warp_part[threadIdx.x].x, warp_part[threadIdx.x].y);
-                all.merge_warp();
+                RowAnswer r;
+                if (o.says_nothing()) r = row_answer(top_by_warp<DT>(x, a.vocab), E::up(x[y]), c, a.inv_temperature);
+                else r = row_answer<false>(o, E::up(x[y]), c);
                 if (threadIdx.x == 0) {
-                    const RowAnswer r = row_answer(all, E::up(x[y]), c);
                     a.logp[row] = r.logp;
                     if (a.lse) a.lse[row] = r.lse;
                     if (MODE == kModePolicy) {
                         const float k = policy_term(p, r.logp, row).coef * S * a.inv_temperature;
-                        answer = make_float4(r.e, -k * r.inv, -k * expm1f(r.logp), 0.0f);
+                        answer = make_float4(r.e, -k * r.inv, -k * expm1f(r.logp), r.by);
                     }
                 }
             }
@@ -289,14 +381,15 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
         if (MODE == kModeLogprob) continue;
 
         // gradient
-        float e, kn, ky;
+        float e, kn, ky, by = c;
         if (MODE == kModePolicy) {
             e = answer.x;
             kn = answer.y;
             ky = answer.z;
+            by = answer.w;
         } else {
             // 2^(c z - log2e lse) = 2^(c z - e) * 2^(e - log2e lse), e an integer
-            const float lse = lse_in[row], k = coef_in[row] * S * a.inv_temperature;
+            const float lse = usable(lse_in[row]), k = coef_in[row] * S * a.inv_temperature;
             const bool empty = lse == -INFINITY;
             e = empty ? 0.0f : rintf(lse * kLog2E);
             kn = empty ? 0.0f * k : -k * exp2f(-fmaf(lse, kLog2E, -e));
@@ -307,16 +400,16 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
         const bool vec = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
         if (vec) {
             uint4* out = reinterpret_cast<uint4*>(g + cut.head);
-            for (uint32_t i = threadIdx.x; i < cut.groups; i += kRowThreads) __stcs(out + i, grad_group<DT>(body[i], c, e, kn));
+            for (uint32_t i = threadIdx.x; i < cut.groups; i += kRowThreads) __stcs(out + i, grad_group<DT>(body[i], by, e, kn));
             if ((uint32_t)y - cut.head < cut.groups * E::kVec && ((uint32_t)y - cut.head) / E::kVec % kRowThreads == threadIdx.x)
                 g[y] = E::down(ky);              // behind this thread's own store of the group
             if (threadIdx.x < cut.head)
-                g[threadIdx.x] = E::down(threadIdx.x == (uint32_t)y ? ky : kn * exp2_fast(fmaf(E::up(x[threadIdx.x]), c, -e)));
+                g[threadIdx.x] = E::down(threadIdx.x == (uint32_t)y ? ky : kn * exp2_fast(fmaf(E::up(x[threadIdx.x]), by, -e)));
             for (uint32_t i = tail + threadIdx.x; i < a.vocab; i += kRowThreads)
-                g[i] = E::down(i == (uint32_t)y ? ky : kn * exp2_fast(fmaf(E::up(x[i]), c, -e)));
+                g[i] = E::down(i == (uint32_t)y ? ky : kn * exp2_fast(fmaf(E::up(x[i]), by, -e)));
         } else {
             for (uint32_t i = threadIdx.x; i < a.vocab; i += kRowThreads)
-                g[i] = E::down(i == (uint32_t)y ? ky : kn * exp2_fast(fmaf(E::up(x[i]), c, -e)));
+                g[i] = E::down(i == (uint32_t)y ? ky : kn * exp2_fast(fmaf(E::up(x[i]), by, -e)));
         }
         __syncthreads();                                  // the shared values are written again for the next row
     }
@@ -386,7 +479,7 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t phase, uint32_
 // barrier and 629 us with this, 4096 x 151936 bf16).
 template <int WARPS>
 struct ClusterSum {
-    float2 part[2][kMostCluster * WARPS];  // (e, s) of each warp of the cluster, by row parity: a CTA may be a row ahead
+    float2 part[2][kMostCluster * WARPS];  // (e, s) of each warp of the cluster, by exchange parity: a CTA may be one ahead
     uint2 next[2];                         // what warp 0 of the first CTA passes on
     unsigned long long bar[2];
 
@@ -406,8 +499,9 @@ struct ClusterSum {
     static __device__ __forceinline__ void cluster_barrier() {
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
-    // every warp, row n (counted from 0): hands what it has of the sum to warp 0 of every CTA
-    __device__ __forceinline__ void give(Online o, uint2 pass_on, uint32_t n, uint32_t rank, uint32_t C) {
+    // every warp, exchange n (counted from 0): hands what it has of the sum to warp 0 of every CTA
+    template <typename Sum>
+    __device__ __forceinline__ void give(Sum o, uint2 pass_on, uint32_t n, uint32_t rank, uint32_t C) {
         const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, parity = n & 1;
         o.merge_warp();
         if (C == 1) {
@@ -432,10 +526,11 @@ struct ClusterSum {
         }
     }
     // warp 0 (C = 1: behind a barrier with all that give): the sum over the cluster
-    __device__ __forceinline__ Online take(float c, uint32_t n, uint32_t C) {
+    template <typename Sum>
+    __device__ __forceinline__ Sum take(float c, uint32_t n, uint32_t C) {
         const uint32_t lane = threadIdx.x & 31, parity = n & 1, phase = (n >> 1) & 1;
         const bool done = C == 1 || wait_phase(smem_at(&bar[parity]), phase);
-        Online o(c);
+        Sum o(c);
         if (!done) {                                         // gave up: the row's results are NaN
             if (lane == 0) {
                 atomicExch(&losses_error_word, 1u);
@@ -510,7 +605,7 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
     __shared__ ClusterSum<THREADS / 32> sums;
     __shared__ RowFeed feed;
     __shared__ float inputs[8];
-    __shared__ float4 answer;                         // e, -k / s, k (1 - p_y)
+    __shared__ float4 answer;                         // e, -k / s, k (1 - p_y), factor of z (policy kernel: 0 for a row to be looked at again)
     const uint32_t C = cooperative_groups::this_cluster().num_blocks(), rank = cooperative_groups::this_cluster().block_rank();
     const int tid = threadIdx.x;
     const bool asks = rank == 0 && tid == 0;
@@ -563,30 +658,33 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
         sums.give(o, next, n, rank, C);
         __syncthreads();
         if (tid < 32) {
-            o = sums.take(c, n, C);
+            o = sums.template take<Online>(c, n, C);
             if (tid == 0 && y < a.vocab) {
-                const RowAnswer r = row_answer(o, inputs[0], c);
-                if (rank == 0) a.logp[row] = r.logp;
+                const RowAnswer r = row_answer<true>(o, inputs[0], c);
+                const bool again = fabsf(o.e) >= kExact || o.says_nothing();
+                if (rank == 0) a.logp[row] = again ? __uint_as_float(kLookAgain) : r.logp;
                 const float S = a.scaler ? a.scaler->scale : 1.0f;
                 const float k = policy_term(p, r.logp, inputs[1], inputs[2], inputs[3], inputs[4]).coef * S * a.inv_temperature;
-                answer = make_float4(r.e, -k * r.inv, -k * expm1f(r.logp), 0.0f);
+                answer = make_float4(r.e, -k * r.inv, -k * expm1f(r.logp), again ? 0.0f : c);
             } else if (asks) {
                 a.logp[row] = 0.0f;
             }
         }
         __syncthreads();
         const float e = answer.x, kn = answer.y, ky = answer.z;
-        // the gradient's groups lie where the logits' do
-        uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(now.in) + reinterpret_cast<uintptr_t>(g) -
-                                              reinterpret_cast<uintptr_t>(now.x));
+        if (answer.w != 0.0f) {                       // (0: the row is left to the kernel behind this one)
+            // the gradient's groups lie where the logits' do
+            uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(now.in) + reinterpret_cast<uintptr_t>(g) -
+                                                  reinterpret_cast<uintptr_t>(now.x));
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            // the packed group is what stays in registers, not what the sum unpacked from it
-            asm volatile("" : "+r"(v[j].x), "+r"(v[j].y), "+r"(v[j].z), "+r"(v[j].w));
-            if (j < (int)now.groups) __stcs(out + j * THREADS, grad_group<DT>(v[j], c, e, kn));
+            for (int j = 0; j < NV; j++) {
+                // the packed group is what stays in registers, not what the sum unpacked from it
+                asm volatile("" : "+r"(v[j].x), "+r"(v[j].y), "+r"(v[j].z), "+r"(v[j].w));
+                if (j < (int)now.groups) __stcs(out + j * THREADS, grad_group<DT>(v[j], c, e, kn));
+            }
+            if (now.end_at < a.vocab) g[now.end_at] = E::down(now.end_at == y ? ky : kn * exp2_fast(fmaf(end, c, -e)));
+            if (now.owns_y) g[y] = E::down(ky);           // behind this thread's own store of the group
         }
-        if (now.end_at < a.vocab) g[now.end_at] = E::down(now.end_at == y ? ky : kn * exp2_fast(fmaf(end, c, -e)));
-        if (now.owns_y) g[y] = E::down(ky);           // behind this thread's own store of the group
         row = sums.next[n & 1].x;
         y = sums.next[n & 1].y;
         if (row >= a.rows) break;
@@ -644,11 +742,15 @@ logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
     sums.give(o, make_uint2(0u, 0u), 0, rank, C);
     __syncthreads();
     if (tid < 32) {
-        o = sums.take(c, 0, C);
-        if (tid == 0 && rank == 0) {
-            const RowAnswer r = row_answer(o, z_y, c);
-            a.logp[row] = r.logp;
-            if (a.lse) a.lse[row] = r.lse;
+        o = sums.template take<Online>(c, 0, C);
+        if (rank == 0) {
+            RowAnswer r;
+            if (__shfl_sync(0xFFFFFFFFu, o.says_nothing(), 0)) r = row_answer(top_by_warp<DT>(now.x, a.vocab), z_y, c, a.inv_temperature);
+            else r = row_answer<false>(o, z_y, c);
+            if (tid == 0) {
+                a.logp[row] = r.logp;
+                if (a.lse) a.lse[row] = r.lse;
+            }
         }
     }
     sums.finish(C);
@@ -667,7 +769,7 @@ logits_grad_kernel(LogitsArgs a, const float* lse_in, const float* coef_in, uint
     const uint32_t row = blockIdx.x / runs, run = blockIdx.x - row * runs;
     const uint32_t tid = threadIdx.x;
     const int32_t y = a.targets[row];
-    const float coef = coef_in[row], lse = lse_in[row], S = a.scaler ? a.scaler->scale : 1.0f;
+    const float coef = coef_in[row], lse = usable(lse_in[row]), S = a.scaler ? a.scaler->scale : 1.0f;
     const T* x = static_cast<const T*>(a.data) + (uint64_t)row * a.row_stride;
     T* g = static_cast<T*>(a.grad) + (uint64_t)row * a.grad_stride;
     const RowCut cut = cut_row(x, a.vocab);
@@ -730,24 +832,62 @@ struct PolicySums {
     }
 };
 
-// Weighted sums of the policy loss over all tokens, and the gradient by log-probability.  `targets` (with vocab):
-// tokens whose target is out of range take no part.  One cluster: its CTAs hand their sums to the first one, so the
+// A row that logits_policy_kernel has marked, by the whole CTA: log-probability and gradient.  It happens to rows of nothing
+// but masks and to logits beyond 2^31, so it is written to be short; in the kernel that marks it, it cost registers and with
+// them 7 to 14 % of every call.
+template <uint32_t DT>
+__device__ __noinline__ void look_again(const LogitsArgs& a, const PolicyArgs& p, uint64_t row) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    __shared__ float2 parts[kVectorThreads / 32];
+    __shared__ RowAnswer answer;
+    const T* x = static_cast<const T*>(a.data) + row * a.row_stride;
+    T* g = static_cast<T*>(a.grad) + row * a.grad_stride;
+    const uint32_t y = (uint32_t)a.targets[row];
+    const float c = a.inv_temperature * kLog2E;
+    Online o(c);
+    for (uint32_t i = threadIdx.x; i < a.vocab; i += kVectorThreads) o.add(E::up(x[i]), c);
+    o = add_in_block(o, parts, c);
+    if (o.says_nothing()) {
+        __syncthreads();
+        Top top;
+        for (uint32_t i = threadIdx.x; i < a.vocab; i += kVectorThreads) top.add(E::up(x[i]));
+        top = add_in_block(top, parts, c);
+        if (threadIdx.x == 0) answer = row_answer(top, E::up(x[y]), c, a.inv_temperature);
+    } else if (threadIdx.x == 0) {
+        answer = row_answer<false>(o, E::up(x[y]), c);
+    }
+    __syncthreads();
+    const RowAnswer r = answer;
+    const float k = policy_term(p, r.logp, row).coef * (a.scaler ? a.scaler->scale : 1.0f) * a.inv_temperature;
+    for (uint32_t i = threadIdx.x; i < a.vocab; i += kVectorThreads)
+        g[i] = E::down(i == y ? -k * expm1f(r.logp) : -k * r.inv * exp2_fast(fmaf(E::up(x[i]), r.by, -r.e)));
+    if (threadIdx.x == 0) a.logp[row] = r.logp;
+    __syncthreads();
+}
+
+// Weighted sums of the policy loss over all tokens, and the gradient by log-probability.  `a` (with targets): tokens whose
+// target is out of range take no part, rows marked by logits_policy_kernel are done first.  One cluster: its CTAs hand their sums to the first one, so the
 // record needs no scratch memory and no second launch.  Bound by latency: 16384 tokens 4.5 us in a graph.
 __global__ void __launch_bounds__(kVectorThreads)
-policy_kernel(const float* logp, uint64_t tokens, const int32_t* targets, uint32_t vocab, PolicyArgs p, float* coef,
-              rlcu_policy_stat* stat, uint32_t flags) {
+policy_kernel(const float* logp, uint64_t tokens, const __grid_constant__ LogitsArgs a, uint32_t dtype,
+              const __grid_constant__ PolicyArgs p, float* coef, rlcu_policy_stat* stat, uint32_t flags) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ PolicySums warps[kVectorThreads / 32], ctas[kMostCluster];
     const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
     asm volatile("griddepcontrol.wait;" ::: "memory");
+sums:
     PolicySums mine;
+    bool marked = false;                              // a row that logits_policy_kernel has left is among the CTA's
     for (uint64_t t = rank * kVectorThreads + threadIdx.x; t < tokens; t += C * kVectorThreads) {
         const float w = p.weight[t];
-        const bool takes = w != 0.0f && (!targets || (targets[t] >= 0 && (uint32_t)targets[t] < vocab));
+        const bool takes = w != 0.0f && (!a.targets || (a.targets[t] >= 0 && (uint32_t)a.targets[t] < a.vocab));
         float co = 0.0f;
         if (takes) {
-            const PolicyTerm o = policy_term(p, logp[t], t);
+            const float lp = logp[t];
+            if (a.grad) marked |= __float_as_uint(lp) == kLookAgain;
+            const PolicyTerm o = policy_term(p, lp, t);
             mine.l += (double)w * o.l;
             mine.k += (double)w * o.k;
             mine.w += w;
@@ -760,7 +900,15 @@ policy_kernel(const float* logp, uint64_t tokens, const int32_t* targets, uint32
     }
     mine.add_warp();
     if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = mine;
-    __syncthreads();
+    if (__syncthreads_or(marked)) {
+        for (uint64_t t = rank * kVectorThreads; t < tokens; t += t % kVectorThreads == kVectorThreads - 1 ? (C - 1) * kVectorThreads + 1 : 1) {
+            if (__float_as_uint(logp[t]) != kLookAgain) continue;       // (one thread changes it, behind a barrier all pass)
+            if (dtype == RLCU_F16) look_again<RLCU_F16>(a, p, t);
+            else if (dtype == RLCU_BF16) look_again<RLCU_BF16>(a, p, t);
+            else look_again<RLCU_F32>(a, p, t);
+        }
+        goto sums;
+    }
     if (threadIdx.x < 32) {
         mine = warps[threadIdx.x];
         mine.add_warp();
@@ -1164,8 +1312,8 @@ int launch_grad(const LogitsArgs& a, uint32_t dtype, const float* lse, const flo
 }
 
 // behind: launched while the call's own kernel before it still runs (policy_kernel waits for its end)
-int launch_policy(const float* logp, uint64_t tokens, const int32_t* targets, uint32_t vocab, const PolicyArgs& p,
-                  float* coef, rlcu_policy_stat* stat, uint32_t flags, bool behind, cudaStream_t s) {
+int launch_policy(const float* logp, uint64_t tokens, const LogitsArgs& a, uint32_t dtype, const PolicyArgs& p, float* coef,
+                  rlcu_policy_stat* stat, uint32_t flags, bool behind, cudaStream_t s) {
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg = cluster_launch(attr, tokens <= kVectorThreads ? 1 : tokens <= 4 * kVectorThreads ? 4 : 8, kVectorThreads, s);
     if (behind) {
@@ -1173,7 +1321,7 @@ int launch_policy(const float* logp, uint64_t tokens, const int32_t* targets, ui
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = 2;
     }
-    RLCU_CUDA(cudaLaunchKernelEx(&cfg, policy_kernel, logp, tokens, targets, vocab, p, coef, stat, flags));
+    RLCU_CUDA(cudaLaunchKernelEx(&cfg, policy_kernel, logp, tokens, a, dtype, p, coef, stat, flags));
     return RLCU_OK;
 }
 
@@ -1214,7 +1362,7 @@ extern "C" int rlcu_policy_loss_logp(const float* logp, uint64_t tokens, const f
     if (!out_apart(coef, tokens, {logp, old_logp, ref_logp, advantage, weight}, true))
         return set_error(RLCU_ERR_INVALID, "coef overlaps an input without being the same buffer");
     PolicyArgs p = {old_logp, ref_logp, advantage, weight, *hp};
-    return launch_policy(logp, tokens, nullptr, 0, p, coef, stat, flags, false, (cudaStream_t)stream);
+    return launch_policy(logp, tokens, LogitsArgs{}, RLCU_F32, p, coef, stat, flags, false, (cudaStream_t)stream);
 }
 
 extern "C" int rlcu_policy_loss(const void* logits, uint32_t dtype, uint64_t rows, uint64_t vocab, uint64_t row_stride,
@@ -1238,7 +1386,7 @@ extern "C" int rlcu_policy_loss(const void* logits, uint32_t dtype, uint64_t row
                             : launch_logits<kModeLogprob>(a, p, dtype, (cudaStream_t)stream);
         if (rc) return rc;
     }
-    return launch_policy(logp, rows, targets, (uint32_t)vocab, p, nullptr, stat, flags, rows > 0, (cudaStream_t)stream);
+    return launch_policy(logp, rows, a, dtype, p, nullptr, stat, flags, rows > 0, (cudaStream_t)stream);
 }
 
 extern "C" int rlcu_preference_loss(const float* logp, uint64_t tokens, const float* ref_logp, const uint8_t* mask,
