@@ -1,0 +1,53 @@
+"""GPU tests of the records of the losses where a cluster has CTAs with little or no work: the ones that are done at once
+hand their sums to a first CTA that must have started."""
+import pytest
+import torch
+
+import operator_oracle as Q
+from test_losses_gpu import check_preference, off_the_borders, stat_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("tokens", [1025, 1500, 2048, 3072, 4097, 9000])
+def test_policy_records_of_clusters_with_idle_ctas(pkg, tokens):
+    g = torch.Generator().manual_seed(tokens)
+    logp = -torch.rand(tokens, generator=g) * 3
+    old = logp - off_the_borders(torch.randn(tokens, generator=g) * 0.3, 0.2, 0.2, 0.0)
+    a, w = torch.randn(tokens, generator=g), torch.rand(tokens, generator=g)
+    hp = pkg.policy_hparams(0.2, 0.2)
+    d = [t.cuda() for t in (logp, a, w, old)]
+    per = Q.policy(logp, old, None, a, w, w != 0, float(torch.tensor(0.2)), float(torch.tensor(0.2)), 0.0, 0.0, 3)
+    wl = w.to(Q.F64) * per[0]
+    e = Q.policy_error(torch.zeros(tokens, dtype=Q.F64), old, None, logp, a, w, w != 0, 0.0)
+    records = torch.full((200, 8), 0x7FC00000, dtype=torch.int32, device="cuda")
+    for k in range(200):
+        pkg.policy_loss_logp(d[0].data_ptr(), tokens, d[1].data_ptr(), d[2].data_ptr(), hp, records[k].data_ptr(), None, d[3].data_ptr())
+    torch.cuda.synchronize()
+    assert bool((records == records[0]).all())
+    s = stat_of(pkg.PolicyStat, records[0])
+    assert (s.tokens, s.clipped) == (tokens, int(per[3].sum()))
+    assert abs(s.loss - float(wl.sum())) <= float(e.sum()) + float(wl.abs().sum()) * 2.0 ** -20
+
+
+@pytest.mark.parametrize("pairs,tokens", [(3, 40000), (5, 40000), (9, 70000), (3, 9000)])
+def test_preference_records_of_clusters_with_idle_ctas(pkg, pairs, tokens):
+    """More CTAs than pairs (their number is a power of two), without coefficients to write."""
+    g = torch.Generator().manual_seed(pairs)
+    cuts = torch.randint(0, tokens + 1, (2 * pairs - 1,), generator=g).sort().values.tolist()
+    offsets = [0] + cuts + [tokens]
+    check_preference(pkg, offsets, tokens, pairs, mask=False)
+    logp, ob = -torch.rand(tokens, generator=g).cuda(), torch.tensor(offsets, dtype=torch.int32).cuda()
+    records = torch.full((200, 8), 0x7FC00000, dtype=torch.int32, device="cuda")
+    hp = pkg.preference_hparams(0.1)
+    for k in range(200):
+        pkg.preference_loss(logp.data_ptr(), tokens, ob.data_ptr(), pairs, hp, records[k].data_ptr())
+    torch.cuda.synchronize()
+    assert bool((records == records[0]).all())
+    beta = float(torch.tensor(0.1))
+    sums = torch.stack([logp.cpu().to(Q.F64)[lo:hi].sum() for lo, hi in zip(offsets, offsets[1:])]).view(pairs, 2)
+    h = beta * (sums[:, 0] - sums[:, 1])
+    loss, margin = float(torch.nn.functional.softplus(-h, threshold=1e9).mean()), float(h.mean())
+    s = stat_of(pkg.PreferenceStat, records[0])
+    assert (s.pairs, s.correct) == (pairs, int((sums[:, 0] > sums[:, 1]).sum()))
+    assert abs(s.loss - loss) <= abs(loss) * 2.0 ** -20 and abs(s.margin - margin) <= abs(margin) * 2.0 ** -20
