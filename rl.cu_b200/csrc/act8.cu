@@ -643,7 +643,8 @@ __device__ __forceinline__ void set_four(Run<DT>& r, int i, const F2 (&p)[2]) {
 
 // The end of a gradient kernel whose grid is one cluster: partial sums added in order, the columns dealt to all threads.
 __device__ __forceinline__ void add_parts_in_cluster(const NormArgs& a) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // (not .aligned: the threads of a warp come from different branches)
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
     for (uint32_t j = blockIdx.x * blockDim.x + threadIdx.x; j < a.cols; j += gridDim.x * blockDim.x) {
         float s = 0.0f;
         for (uint32_t p = 0; p < gridDim.x; p++) s += __ldcg(a.partial + (uint64_t)p * a.cols + j);

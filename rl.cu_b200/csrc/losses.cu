@@ -496,8 +496,9 @@ struct ClusterSum {
     __device__ __forceinline__ void finish(uint32_t C) {
         if (C > 1) cluster_barrier();
     }
+    // (not .aligned: the threads of a warp come from different branches)
     static __device__ __forceinline__ void cluster_barrier() {
-        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
     }
     // every warp, exchange n (counted from 0): hands what it has of the sum to warp 0 of every CTA
     template <typename Sum>
