@@ -144,13 +144,21 @@ int rlcu_preference_loss(const float* logp, uint64_t tokens, const float* ref_lo
                          rlcu_preference_stat* stat, uint32_t flags, void* stream);
 
 /* -------- bounded waits ------------------------------------------------------ */
-/* The CTAs that share a row of logits wait for one another, for a bounded time.  Waits for every stream of the
- * device (cudaDeviceSynchronize) and reports whether such a wait gave up since the last check
- * (RLCU_ERR_TIMEOUT: the results of that call are incomplete, the rows concerned are NaN).  Clears the condition. */
+/* The CTAs that share a row of logits wait for one another, for a bounded time.  When such a wait gives up
+ *   - rlcu_token_logprob: log-probability (and lse) of the rows concerned may be NaN;
+ *   - rlcu_policy_loss: rows may have been left out.  All log-probabilities of the call, the first value of each row of its
+ *     gradient (which rlcu_gradstat finds) and loss, policy and weight of its record are NaN; so are those of later
+ *     calls of rlcu_policy_loss on the device until the condition is cleared.
+ * Waits for every stream of the device (cudaDeviceSynchronize), reports whether a wait gave up since the last check
+ * (RLCU_ERR_TIMEOUT) and clears the condition. */
 int rlcu_losses_check(void);
 /* Runs a one-thread kernel whose bounded wait is certain to run out and reports it through the same path: the
  * expected return value is RLCU_ERR_TIMEOUT, and the device stays usable. */
 int rlcu_losses_selftest_wait(void* stream);
+/* For tests: how often the waits of kernels launched later by this process try before they count as given up (they wait on
+ * after that, so that nothing is left on its way; the results are spoilt all the same).  0: at once.  More than the
+ * number they start with counts as that number.  Returns the number that held before. */
+uint32_t rlcu_losses_selftest_tries(uint32_t tries);
 
 #ifdef __cplusplus
 }

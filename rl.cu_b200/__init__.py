@@ -45,7 +45,7 @@ EXPORTS = [
     "rlcu_zero1_step", "rlcu_zero1_poll_error", "rlcu_zero1_check", "rlcu_zero1_destroy",
     "rlcu_checkpoint_save", "rlcu_checkpoint_peek", "rlcu_checkpoint_load",
     "rlcu_token_logprob", "rlcu_token_logprob_grad", "rlcu_policy_loss", "rlcu_policy_loss_logp", "rlcu_preference_loss",
-    "rlcu_losses_check", "rlcu_losses_selftest_wait",
+    "rlcu_losses_check", "rlcu_losses_selftest_wait", "rlcu_losses_selftest_tries",
     "rlcu_act8_blocks", "rlcu_act8_store", "rlcu_act8_load", "rlcu_act8_rmsnorm", "rlcu_act8_rmsnorm_grad_workspace",
     "rlcu_act8_rmsnorm_grad",
 ]
@@ -209,6 +209,8 @@ def lib() -> C.CDLL:
     L.rlcu_preference_loss.argtypes = [vp, u64, vp, vp, vp, u64, vp, vp, vp, vp, vp, u32, vp]
     L.rlcu_losses_check.argtypes = []
     L.rlcu_losses_selftest_wait.argtypes = [vp]
+    L.rlcu_losses_selftest_tries.argtypes = [u32]
+    L.rlcu_losses_selftest_tries.restype = u32
     L.rlcu_act8_blocks.argtypes = [u64]
     L.rlcu_act8_blocks.restype = u64
     L.rlcu_act8_store.argtypes = [vp, u32, u64, u64, u64, vp, u64, vp, vp]
@@ -473,6 +475,11 @@ def losses_check():
 def losses_selftest_wait(stream=None) -> int:
     """Status of a wait that is certain to run out (``ERR_TIMEOUT``)."""
     return lib().rlcu_losses_selftest_wait(stream)
+
+
+def losses_selftest_tries(tries) -> int:
+    """Tries of the waits of later launches before they count as given up; returns the number that held before."""
+    return lib().rlcu_losses_selftest_tries(tries)
 
 
 # ---------------------------------------------------------------------------

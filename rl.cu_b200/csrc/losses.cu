@@ -9,6 +9,7 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 
@@ -41,6 +42,7 @@ struct LogitsArgs {
     void* grad;
     uint64_t grad_stride;
     const rlcu_scaler_state* scaler;
+    uint32_t tries;           // of a wait before it counts as given up
 };
 
 struct PolicyArgs {
@@ -452,8 +454,8 @@ struct RowShare {
     }
 };
 
-// Set when a bounded wait below gave up; read and cleared by rlcu_losses_check.  In host code this name is only a
-// handle for cudaMemcpyFromSymbol.
+// Set when a bounded wait below gave up; read by policy_kernel, read and cleared by rlcu_losses_check.  In host code this
+// name is only a handle for cudaMemcpyFromSymbol.
 static __device__ unsigned int losses_error_word;
 constexpr uint32_t kWaitTries = 1u << 18;
 
@@ -471,6 +473,14 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t phase, uint32_
             "}\n"
             : "=r"(done) : "r"(bar), "r"(phase) : "memory");
     return done;
+}
+
+// A wait that gave up says so and is taken up again, once: what is on its way to this CTA should not arrive after it has
+// left.  False: it has not arrived in that time either.
+__device__ __forceinline__ bool wait_or_say(uint32_t bar, uint32_t phase, uint32_t tries) {
+    if (wait_phase(bar, phase, tries)) return true;
+    atomicExch(&losses_error_word, 1u);
+    return wait_phase(bar, phase);
 }
 
 // Sums of all threads of a cluster, in warp 0 of each of its CTAs.  The CTAs hand each other their sums with st.async,
@@ -528,15 +538,12 @@ struct ClusterSum {
     }
     // warp 0 (C = 1: behind a barrier with all that give): the sum over the cluster
     template <typename Sum>
-    __device__ __forceinline__ Sum take(float c, uint32_t n, uint32_t C) {
+    __device__ __forceinline__ Sum take(float c, uint32_t n, uint32_t C, uint32_t tries) {
         const uint32_t lane = threadIdx.x & 31, parity = n & 1, phase = (n >> 1) & 1;
-        const bool done = C == 1 || wait_phase(smem_at(&bar[parity]), phase);
+        const bool done = C == 1 || __all_sync(0xFFFFFFFFu, wait_or_say(smem_at(&bar[parity]), phase, tries));
         Sum o(c);
-        if (!done) {                                         // gave up: the row's results are NaN
-            if (lane == 0) {
-                atomicExch(&losses_error_word, 1u);
-                next[parity] = make_uint2(0xFFFFFFFFu, 0u);
-            }
+        if (!done) {                                         // no more rows for this CTA
+            if (lane == 0) next[parity] = make_uint2(0xFFFFFFFFu, 0u);
             o.s = NAN;
         } else {
             for (uint32_t i = lane; i < C * WARPS; i += 32) o.merge(part[parity][i].x, part[parity][i].y);
@@ -565,11 +572,8 @@ struct RowFeed {
                      :: "r"(smem_at(&response)), "r"(smem_at(&bar)) : "memory");
     }
     // first CTA of the cluster taken over by request n (counted from 0), or -1: none was left
-    __device__ __forceinline__ int answer(uint32_t n) {
-        if (!wait_phase(smem_at(&bar), n & 1)) {
-            atomicExch(&losses_error_word, 1u);
-            return -1;
-        }
+    __device__ __forceinline__ int answer(uint32_t n, uint32_t tries) {
+        if (!wait_or_say(smem_at(&bar), n & 1, tries)) return -1;
         unsigned long long lo, hi;
         int first;
         asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(smem_at(&response)) : "memory");
@@ -641,7 +645,7 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
         for (int j = 0; j < NV; j++) {
             if (j < (int)now.groups) o.add<DT>(v[j], c);
             if (j == 0 && asks) {
-                const int first = feed.answer(n);
+                const int first = feed.answer(n, a.tries);
                 if (first >= 0) {
                     next.x = (uint32_t)first / C;
                     next.y = (uint32_t)a.targets[next.x];
@@ -659,7 +663,7 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
         sums.give(o, next, n, rank, C);
         __syncthreads();
         if (tid < 32) {
-            o = sums.template take<Online>(c, n, C);
+            o = sums.template take<Online>(c, n, C, a.tries);
             if (tid == 0 && y < a.vocab) {
                 const RowAnswer r = row_answer<true>(o, inputs[0], c);
                 const bool again = fabsf(o.e) >= kExact || o.says_nothing();
@@ -743,7 +747,7 @@ logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
     sums.give(o, make_uint2(0u, 0u), 0, rank, C);
     __syncthreads();
     if (tid < 32) {
-        o = sums.template take<Online>(c, 0, C);
+        o = sums.template take<Online>(c, 0, C, a.tries);
         if (rank == 0) {
             RowAnswer r;
             if (__shfl_sync(0xFFFFFFFFu, o.says_nothing(), 0)) r = row_answer(top_by_warp<DT>(now.x, a.vocab), z_y, c, a.inv_temperature);
@@ -872,9 +876,19 @@ __device__ __noinline__ void look_again(const LogitsArgs& a, const PolicyArgs& p
     __syncthreads();
 }
 
+// log-probability and first gradient of a row as NaN
+__device__ __forceinline__ void spoil(const LogitsArgs& a, uint32_t dtype, uint64_t row) {
+    a.logp[row] = NAN;
+    if (!a.grad) return;
+    const uint64_t at = row * a.grad_stride;
+    if (dtype == RLCU_F32) static_cast<float*>(a.grad)[at] = NAN;
+    else static_cast<uint16_t*>(a.grad)[at] = 0x7FFFu;           // (in both 16-bit types)
+}
+
 // Weighted sums of the policy loss over all tokens, and the gradient by log-probability.  `a` (with targets): tokens whose
-// target is out of range take no part, rows marked by logits_policy_kernel are done first.  One cluster: its CTAs hand their sums to the first one, so the
-// record needs no scratch memory and no second launch.  Bound by latency: 16384 tokens 4.8 us in a graph.
+// target is out of range take no part; rows marked by logits_policy_kernel are done first; and after a wait of that kernel
+// has given up, when rows may have been left out, nothing of the call is left that looks like a result.  One cluster: its
+// CTAs hand their sums to the first one, so the record needs no scratch memory and no second launch.  Bound by latency: 16384 tokens 4.8 us in a graph.
 __global__ void __launch_bounds__(kVectorThreads)
 policy_kernel(const float* logp, uint64_t tokens, const __grid_constant__ LogitsArgs a, uint32_t dtype,
               const __grid_constant__ PolicyArgs p, float* coef, rlcu_policy_stat* stat, uint32_t flags) {
@@ -884,6 +898,7 @@ policy_kernel(const float* logp, uint64_t tokens, const __grid_constant__ Logits
     const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
     cluster_started();
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const bool gave_up = a.targets && *const_cast<const volatile unsigned int*>(&losses_error_word);
 sums:
     PolicySums mine;
     bool marked = false;                              // a row that logits_policy_kernel has left is among the CTA's
@@ -907,14 +922,20 @@ sums:
     }
     mine.add_warp();
     if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = mine;
-    if (__syncthreads_or(marked)) {
-        for (uint64_t t = rank * kVectorThreads; t < tokens; t += t % kVectorThreads == kVectorThreads - 1 ? (C - 1) * kVectorThreads + 1 : 1) {
-            if (__float_as_uint(logp[t]) != kLookAgain) continue;       // (one thread changes it, behind a barrier all pass)
-            if (dtype == RLCU_F16) look_again<RLCU_F16>(a, p, t);
-            else if (dtype == RLCU_BF16) look_again<RLCU_BF16>(a, p, t);
-            else look_again<RLCU_F32>(a, p, t);
+    if (__syncthreads_or(marked || gave_up)) {
+        if (__syncthreads_or(gave_up)) {
+            for (uint64_t t = rank * kVectorThreads + threadIdx.x; t < tokens; t += C * kVectorThreads) spoil(a, dtype, t);
+            if (threadIdx.x == 0) warps[0].l = warps[0].w = NAN;
+            __syncthreads();
+        } else {
+            for (uint64_t t = rank * kVectorThreads; t < tokens; t += t % kVectorThreads == kVectorThreads - 1 ? (C - 1) * kVectorThreads + 1 : 1) {
+                if (__float_as_uint(logp[t]) != kLookAgain) continue;   // (one thread changes it, behind a barrier all pass)
+                if (dtype == RLCU_F16) look_again<RLCU_F16>(a, p, t);
+                else if (dtype == RLCU_BF16) look_again<RLCU_BF16>(a, p, t);
+                else look_again<RLCU_F32>(a, p, t);
+            }
+            goto sums;
         }
-        goto sums;
     }
     wait_cluster_started();
     if (threadIdx.x < 32) {
@@ -1214,6 +1235,8 @@ bool out_apart(const float* out, uint64_t n, std::initializer_list<const float*>
     return true;
 }
 
+std::atomic<uint32_t> wait_tries{kWaitTries};
+
 int sm_count(int* out) {
     int dev = 0;
     RLCU_CUDA(cudaGetDevice(&dev));
@@ -1346,7 +1369,7 @@ extern "C" int rlcu_token_logprob(const void* logits, uint32_t dtype, uint64_t r
     if (rows && !logp) return set_error(RLCU_ERR_INVALID, "null logp");
     if (!words_aligned({targets, logp, lse})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
     if (!rows) return RLCU_OK;
-    LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, logp, lse, nullptr, 0, nullptr};
+    LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, logp, lse, nullptr, 0, nullptr, wait_tries};
     return launch_logits<kModeLogprob>(a, PolicyArgs{}, dtype, (cudaStream_t)stream);
 }
 
@@ -1359,7 +1382,7 @@ extern "C" int rlcu_token_logprob_grad(const void* logits, uint32_t dtype, uint6
     if (rows && (!lse || !coef)) return set_error(RLCU_ERR_INVALID, "null lse or coef");
     if (!words_aligned({targets, lse, coef, scaler})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
     if (!rows) return RLCU_OK;
-    LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, nullptr, nullptr, grad, grad_stride, scaler};
+    LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, nullptr, nullptr, grad, grad_stride, scaler, wait_tries};
     return launch_grad(a, dtype, lse, coef, (cudaStream_t)stream);
 }
 
@@ -1389,7 +1412,7 @@ extern "C" int rlcu_policy_loss(const void* logits, uint32_t dtype, uint64_t row
     // logp is written before the record is formed from the inputs
     if (!out_apart(logp, rows, {old_logp, ref_logp, advantage, weight}, false))
         return set_error(RLCU_ERR_INVALID, "logp overlaps another input of the loss");
-    LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, logp, nullptr, grad, grad_stride, scaler};
+    LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, logp, nullptr, grad, grad_stride, scaler, wait_tries};
     PolicyArgs p = {old_logp, ref_logp, advantage, weight, *hp};
     if (rows) {
         const int rc = grad ? launch_logits<kModePolicy>(a, p, dtype, (cudaStream_t)stream)
@@ -1436,6 +1459,8 @@ extern "C" int rlcu_losses_check(void) {
     RLCU_CUDA(cudaMemcpyToSymbol(losses_error_word, &none, sizeof none));
     return set_error(RLCU_ERR_TIMEOUT, "a bounded wait inside a loss kernel gave up: its results are incomplete");
 }
+
+extern "C" uint32_t rlcu_losses_selftest_tries(uint32_t tries) { return wait_tries.exchange(tries < kWaitTries ? tries : kWaitTries); }
 
 extern "C" int rlcu_losses_selftest_wait(void* stream) {
     wait_probe_kernel<<<1, 1, 0, (cudaStream_t)stream>>>();
