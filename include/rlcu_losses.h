@@ -21,7 +21,8 @@
  *
  * Gradients are those of the loss times scaler->scale (the loss scale the statistics pass later divides out;
  * no scaler: 1), rounded once to the logits' type.  A gradient buffer may be the logits' own
- * (same pointer, same stride); any other overlap is refused.
+ * (same pointer, same stride).  What a call writes may share no other byte with what it reads or writes elsewhere, unless a
+ * parameter says so; such calls are refused.
  */
 #ifndef RLCU_LOSSES_H
 #define RLCU_LOSSES_H

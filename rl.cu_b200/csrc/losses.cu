@@ -1235,6 +1235,9 @@ bool out_apart(const float* out, uint64_t n, std::initializer_list<const float*>
     return true;
 }
 
+// a vector of 4-byte values
+Span words(const void* p, uint64_t n) { return bytes_of(p, n * 4); }
+
 std::atomic<uint32_t> wait_tries{kWaitTries};
 
 int sm_count(int* out) {
@@ -1369,6 +1372,10 @@ extern "C" int rlcu_token_logprob(const void* logits, uint32_t dtype, uint64_t r
     if (rows && !logp) return set_error(RLCU_ERR_INVALID, "null logp");
     if (!words_aligned({targets, logp, lse})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
     if (!rows) return RLCU_OK;
+    for (const float* out : {logp, lse})
+        if (overlaps_any(words(out, rows), {words(targets, rows), words(out == logp ? lse : logp, rows)}) ||
+            overlaps_rows(words(out, rows), logits, rows, vocab, row_stride, dtype_bytes(dtype)))
+            return set_error(RLCU_ERR_INVALID, "logp or lse overlaps another buffer of the call");
     LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, logp, lse, nullptr, 0, nullptr, wait_tries};
     return launch_logits<kModeLogprob>(a, PolicyArgs{}, dtype, (cudaStream_t)stream);
 }
@@ -1382,6 +1389,9 @@ extern "C" int rlcu_token_logprob_grad(const void* logits, uint32_t dtype, uint6
     if (rows && (!lse || !coef)) return set_error(RLCU_ERR_INVALID, "null lse or coef");
     if (!words_aligned({targets, lse, coef, scaler})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
     if (!rows) return RLCU_OK;
+    for (const Span& in : {words(targets, rows), words(lse, rows), words(coef, rows), bytes_of(scaler, sizeof *scaler)})
+        if (overlaps_rows(in, grad, rows, vocab, grad_stride, dtype_bytes(dtype)))
+            return set_error(RLCU_ERR_INVALID, "gradient overlaps a vector that the call reads");
     LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, nullptr, nullptr, grad, grad_stride, scaler, wait_tries};
     return launch_grad(a, dtype, lse, coef, (cudaStream_t)stream);
 }
@@ -1394,6 +1404,9 @@ extern "C" int rlcu_policy_loss_logp(const float* logp, uint64_t tokens, const f
     if (!words_aligned({logp, old_logp, ref_logp, advantage, weight, coef})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
     if (!out_apart(coef, tokens, {logp, old_logp, ref_logp, advantage, weight}, true))
         return set_error(RLCU_ERR_INVALID, "coef overlaps an input without being the same buffer");
+    if (overlaps_any(bytes_of(stat, sizeof *stat), {words(logp, tokens), words(old_logp, tokens), words(ref_logp, tokens),
+                                                    words(advantage, tokens), words(weight, tokens), words(coef, tokens)}))
+        return set_error(RLCU_ERR_INVALID, "the record overlaps a vector of the call");
     PolicyArgs p = {old_logp, ref_logp, advantage, weight, *hp};
     return launch_policy(logp, tokens, LogitsArgs{}, RLCU_F32, p, coef, stat, flags, false, (cudaStream_t)stream);
 }
@@ -1412,6 +1425,15 @@ extern "C" int rlcu_policy_loss(const void* logits, uint32_t dtype, uint64_t row
     // logp is written before the record is formed from the inputs
     if (!out_apart(logp, rows, {old_logp, ref_logp, advantage, weight}, false))
         return set_error(RLCU_ERR_INVALID, "logp overlaps another input of the loss");
+    const size_t esz = dtype_bytes(dtype);
+    const Span record = bytes_of(stat, sizeof *stat), out = words(logp, rows), scale = bytes_of(scaler, sizeof *scaler);
+    if (overlaps_any(out, {words(targets, rows), scale, record}) || overlaps_rows(out, logits, rows, vocab, row_stride, esz))
+        return set_error(RLCU_ERR_INVALID, "logp overlaps another buffer of the call");
+    for (const Span& v : {words(targets, rows), words(old_logp, rows), words(ref_logp, rows), words(advantage, rows), words(weight, rows), scale, out})
+        if (overlap(v, record) || (grad && overlaps_rows(v, grad, rows, vocab, grad_stride, esz)))
+            return set_error(RLCU_ERR_INVALID, "gradient or record overlaps a vector of the call");
+    if (overlaps_rows(record, logits, rows, vocab, row_stride, esz) || (grad && overlaps_rows(record, grad, rows, vocab, grad_stride, esz)))
+        return set_error(RLCU_ERR_INVALID, "the record overlaps logits or gradient");
     LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, logp, nullptr, grad, grad_stride, scaler, wait_tries};
     PolicyArgs p = {old_logp, ref_logp, advantage, weight, *hp};
     if (rows) {
@@ -1440,6 +1462,12 @@ extern "C" int rlcu_preference_loss(const float* logp, uint64_t tokens, const fl
     if (tokens && !logp) return set_error(RLCU_ERR_INVALID, "null logp");
     if (!words_aligned({logp, ref_logp, offsets, pair_weight, coef, rewards})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
     if (!out_apart(coef, tokens, {logp, ref_logp}, true)) return set_error(RLCU_ERR_INVALID, "coef overlaps an input without being the same buffer");
+    const Span read = bytes_of(mask, tokens), starts = words(offsets, 2 * pairs + 1), weights = words(pair_weight, pairs);
+    const Span record = bytes_of(stat, sizeof *stat), coefs = words(coef, tokens), reward = words(rewards, 2 * pairs);
+    if (overlaps_any(coefs, {read, starts, weights, reward, record}) ||
+        overlaps_any(reward, {words(logp, tokens), words(ref_logp, tokens), read, starts, weights, record}) ||
+        overlaps_any(record, {words(logp, tokens), words(ref_logp, tokens), read, starts, weights}))
+        return set_error(RLCU_ERR_INVALID, "coef, rewards or the record overlaps another buffer of the call");
     PreferenceArgs a = {logp, ref_logp, mask, offsets, pair_weight, tokens, pairs, *hp, coef, rewards, stat, flags};
     // more CTAs than pairs would idle; below a few thousand tokens each, the cluster costs more than it saves
     int cluster = 1;

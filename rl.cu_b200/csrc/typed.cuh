@@ -139,7 +139,25 @@ __host__ inline Span span_of(const void* p, uint64_t rows, uint64_t cols, uint64
     const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
     return {lo, rows && cols ? lo + ((rows - 1) * stride + cols) * esz : lo};
 }
-__host__ inline bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
+__host__ inline bool overlap(Span a, Span b) { return a.lo < a.hi && b.lo < b.hi && a.lo < b.hi && b.lo < a.hi; }
+
+__host__ inline Span bytes_of(const void* p, uint64_t bytes) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+    return {lo, p ? lo + bytes : lo};
+}
+__host__ inline bool overlaps_any(Span a, std::initializer_list<Span> others) {
+    for (const Span& o : others)
+        if (overlap(a, o)) return true;
+    return false;
+}
+// whether v shares a byte with one of the rows of a matrix (what lies between the rows is not the matrix's)
+__host__ inline bool overlaps_rows(Span v, const void* p, uint64_t rows, uint64_t cols, uint64_t stride, size_t esz) {
+    const Span all = span_of(p, rows, cols, stride, esz);
+    if (!overlap(v, all)) return false;
+    if (v.lo <= all.lo) return true;
+    const uint64_t at = v.lo - all.lo, row = at / (stride * esz);
+    return at < row * stride * esz + cols * esz || (row + 1 < rows && v.hi - all.lo > (row + 1) * stride * esz);
+}
 
 // vectors of 4-byte values (null: none), each aligned to them
 __host__ inline bool words_aligned(std::initializer_list<const void*> vectors) {
