@@ -18,6 +18,8 @@
  *   scales : row r at scales + r * rlcu_act8_blocks(cols), one byte per block
  * Decoded values are rounded to the output's type once and, where they are finite, stay finite
  * (RLCU_F16: at most 65504).
+ * What a call writes may share no byte with what it reads or writes elsewhere, unless a parameter says so; such calls are
+ * refused.
  */
 #ifndef RLCU_ACT8_H
 #define RLCU_ACT8_H

@@ -981,6 +981,8 @@ int check_held(const uint8_t* codes, uint64_t& code_stride, const uint8_t* scale
     return RLCU_OK;
 }
 
+Span scales_of(const uint8_t* scales, uint64_t rows, uint64_t cols) { return bytes_of(scales, rows * rlcu_act8_blocks(cols)); }
+
 // the same buffer, or none of it
 bool same_or_apart(const void* p, uint64_t ps, const void* q, uint64_t qs, uint64_t rows, uint64_t cols, size_t esz) {
     if (p == q && (ps == qs || rows <= 1)) return true;
@@ -1124,6 +1126,9 @@ extern "C" int rlcu_act8_store(const void* x, uint32_t dtype, uint64_t rows, uin
     if (!rows || !cols) return RLCU_OK;
     if (overlap(span_of(x, rows, cols, x_stride, dtype_bytes(dtype)), span_of(codes, rows, cols, code_stride, 1)))
         return set_error(RLCU_ERR_INVALID, "x and codes overlap");
+    const Span held = scales_of(scales, rows, cols);
+    if (overlaps_rows(held, x, rows, cols, x_stride, dtype_bytes(dtype)) || overlaps_rows(held, codes, rows, cols, code_stride, 1))
+        return set_error(RLCU_ERR_INVALID, "scales overlap x or codes");
     cudaStream_t s = (cudaStream_t)stream;
     const uint64_t blocks = rlcu_act8_blocks(cols), total = rows * blocks;
     if (rows16(x, x_stride, dtype_bytes(dtype), rows) && rows16(codes, code_stride, 1, rows) && total <= 0x7FFFFFFFull) {
@@ -1152,6 +1157,8 @@ extern "C" int rlcu_act8_load(const uint8_t* codes, uint64_t code_stride, const 
     if (!rows || !cols) return RLCU_OK;
     if (overlap(span_of(x, rows, cols, x_stride, dtype_bytes(dtype)), span_of(codes, rows, cols, code_stride, 1)))
         return set_error(RLCU_ERR_INVALID, "x and codes overlap");
+    if (overlaps_rows(scales_of(scales, rows, cols), x, rows, cols, x_stride, dtype_bytes(dtype)))
+        return set_error(RLCU_ERR_INVALID, "scales and x overlap");
     cudaStream_t s = (cudaStream_t)stream;
     const uint64_t blocks = rlcu_act8_blocks(cols), total = rows * blocks;
     if (rows16(x, x_stride, dtype_bytes(dtype), rows) && rows16(codes, code_stride, 1, rows) && total <= 0x7FFFFFFFull) {
@@ -1185,6 +1192,11 @@ extern "C" int rlcu_act8_rmsnorm(const uint8_t* codes, uint64_t code_stride, con
     if (!rows || !cols) return RLCU_OK;
     if (overlap(span_of(y, rows, cols, y_stride, dtype_bytes(dtype)), span_of(codes, rows, cols, code_stride, 1)))
         return set_error(RLCU_ERR_INVALID, "y and codes overlap");
+    const Span read[] = {scales_of(scales, rows, cols), bytes_of(weight, cols * dtype_bytes(weight_dtype))}, out = bytes_of(rstd, rows * 4);
+    for (const Span& v : {read[0], read[1], out})
+        if (overlaps_rows(v, y, rows, cols, y_stride, dtype_bytes(dtype))) return set_error(RLCU_ERR_INVALID, "y overlaps another buffer of the call");
+    if (overlaps_any(out, {read[0], read[1]}) || overlaps_rows(out, codes, rows, cols, code_stride, 1))
+        return set_error(RLCU_ERR_INVALID, "rstd overlaps another buffer of the call");
     NormArgs a = {codes, code_stride, scales, rows, (uint32_t)cols, (uint32_t)rlcu_act8_blocks(cols), weight, weight_dtype, eps,
                   nullptr, 0, nullptr, 0, y, y_stride, rstd, nullptr, nullptr, 0};
     cudaStream_t s = (cudaStream_t)stream;
@@ -1219,6 +1231,15 @@ extern "C" int rlcu_act8_rmsnorm_grad(const uint8_t* codes, uint64_t code_stride
     if (dweight && need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need))
         return set_error(RLCU_ERR_INVALID, "workspace: %llu bytes, 16-byte aligned, are needed", (unsigned long long)need);
     if (!cols) return RLCU_OK;
+    const Span held = scales_of(scales, rows, cols), w = bytes_of(weight, cols * dtype_bytes(weight_dtype));
+    const Span sums = bytes_of(dweight, cols * 4), parts_at = bytes_of(dweight ? workspace : nullptr, need);
+    for (const Span& v : {held, w, sums, parts_at})
+        if (overlaps_rows(v, dx, rows, cols, dx_stride, esz)) return set_error(RLCU_ERR_INVALID, "dx overlaps another buffer of the call");
+    for (const Span& v : {sums, parts_at})
+        if (overlaps_any(v, {held, w}) || overlaps_rows(v, codes, rows, cols, code_stride, 1) || overlaps_rows(v, dy, rows, cols, dy_stride, esz) ||
+            (dresidual && overlaps_rows(v, dresidual, rows, cols, dresidual_stride, esz)))
+            return set_error(RLCU_ERR_INVALID, "dweight or workspace overlaps what the call reads");
+    if (overlap(sums, parts_at)) return set_error(RLCU_ERR_INVALID, "dweight and workspace overlap");
     cudaStream_t s = (cudaStream_t)stream;
     NormArgs a = {codes, code_stride, scales, rows, (uint32_t)cols, (uint32_t)rlcu_act8_blocks(cols), weight, weight_dtype, eps,
                   dy, dy_stride, dresidual, dresidual_stride, dx, dx_stride, nullptr,
