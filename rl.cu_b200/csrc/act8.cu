@@ -986,7 +986,7 @@ Span scales_of(const uint8_t* scales, uint64_t rows, uint64_t cols) { return byt
 // the same buffer, or none of it
 bool same_or_apart(const void* p, uint64_t ps, const void* q, uint64_t qs, uint64_t rows, uint64_t cols, size_t esz) {
     if (p == q && (ps == qs || rows <= 1)) return true;
-    return !overlap(span_of(p, rows, cols, ps, esz), span_of(q, rows, cols, qs, esz));
+    return !rows_overlap({p, cols * esz, ps * esz}, {q, cols * esz, qs * esz}, rows);
 }
 
 // every row starts on a 16-byte boundary
@@ -1124,7 +1124,7 @@ extern "C" int rlcu_act8_store(const void* x, uint32_t dtype, uint64_t rows, uin
     if (const int rc = check_held(codes, code_stride, scales, rows, cols)) return rc;
     if (const int rc = check_matrix("x", x, dtype, rows, cols, x_stride)) return rc;
     if (!rows || !cols) return RLCU_OK;
-    if (overlap(span_of(x, rows, cols, x_stride, dtype_bytes(dtype)), span_of(codes, rows, cols, code_stride, 1)))
+    if (rows_overlap({x, cols * dtype_bytes(dtype), x_stride * dtype_bytes(dtype)}, {codes, cols, code_stride}, rows))
         return set_error(RLCU_ERR_INVALID, "x and codes overlap");
     const Span held = scales_of(scales, rows, cols);
     if (overlaps_rows(held, x, rows, cols, x_stride, dtype_bytes(dtype)) || overlaps_rows(held, codes, rows, cols, code_stride, 1))
@@ -1155,7 +1155,7 @@ extern "C" int rlcu_act8_load(const uint8_t* codes, uint64_t code_stride, const 
     if (const int rc = check_held(codes, code_stride, scales, rows, cols)) return rc;
     if (const int rc = check_matrix("x", x, dtype, rows, cols, x_stride)) return rc;
     if (!rows || !cols) return RLCU_OK;
-    if (overlap(span_of(x, rows, cols, x_stride, dtype_bytes(dtype)), span_of(codes, rows, cols, code_stride, 1)))
+    if (rows_overlap({x, cols * dtype_bytes(dtype), x_stride * dtype_bytes(dtype)}, {codes, cols, code_stride}, rows))
         return set_error(RLCU_ERR_INVALID, "x and codes overlap");
     if (overlaps_rows(scales_of(scales, rows, cols), x, rows, cols, x_stride, dtype_bytes(dtype)))
         return set_error(RLCU_ERR_INVALID, "scales and x overlap");
@@ -1190,7 +1190,7 @@ extern "C" int rlcu_act8_rmsnorm(const uint8_t* codes, uint64_t code_stride, con
     if (!(eps >= 0.0f) || std::isinf(eps)) return set_error(RLCU_ERR_INVALID, "eps must be finite and not negative");
     if (!words_aligned({rstd})) return set_error(RLCU_ERR_INVALID, "rstd: not aligned to its element size");
     if (!rows || !cols) return RLCU_OK;
-    if (overlap(span_of(y, rows, cols, y_stride, dtype_bytes(dtype)), span_of(codes, rows, cols, code_stride, 1)))
+    if (rows_overlap({y, cols * dtype_bytes(dtype), y_stride * dtype_bytes(dtype)}, {codes, cols, code_stride}, rows))
         return set_error(RLCU_ERR_INVALID, "y and codes overlap");
     const Span read[] = {scales_of(scales, rows, cols), bytes_of(weight, cols * dtype_bytes(weight_dtype))}, out = bytes_of(rstd, rows * 4);
     for (const Span& v : {read[0], read[1], out})
@@ -1225,7 +1225,7 @@ extern "C" int rlcu_act8_rmsnorm_grad(const uint8_t* codes, uint64_t code_stride
     const size_t esz = dtype_bytes(dtype);
     if (!same_or_apart(dx, dx_stride, dy, dy_stride, rows, cols, esz) ||
         (dresidual && !same_or_apart(dx, dx_stride, dresidual, dresidual_stride, rows, cols, esz)) ||
-        overlap(span_of(dx, rows, cols, dx_stride, esz), span_of(codes, rows, cols, code_stride, 1)))
+        rows_overlap({dx, cols * esz, dx_stride * esz}, {codes, cols, code_stride}, rows))
         return set_error(RLCU_ERR_INVALID, "dx overlaps another buffer without being the same");
     const uint64_t need = rlcu_act8_rmsnorm_grad_workspace(rows, cols);
     if (dweight && need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need))

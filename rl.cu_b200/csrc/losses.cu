@@ -1203,7 +1203,7 @@ int check_grad(const void* logits, uint32_t dtype, uint64_t rows, uint64_t vocab
     const size_t esz = dtype_bytes(dtype);
     if (reinterpret_cast<uintptr_t>(grad) % esz) return set_error(RLCU_ERR_INVALID, "gradient not aligned to its element size");
     if (grad == logits && (grad_stride == row_stride || rows <= 1)) return RLCU_OK;
-    if (overlap(span_of(logits, rows, vocab, row_stride, esz), span_of(grad, rows, vocab, grad_stride, esz)))
+    if (rows_overlap({logits, vocab * esz, row_stride * esz}, {grad, vocab * esz, grad_stride * esz}, rows))
         return set_error(RLCU_ERR_INVALID, "gradient and logits overlap without being the same buffer");
     return RLCU_OK;
 }

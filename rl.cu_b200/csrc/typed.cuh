@@ -159,6 +159,20 @@ __host__ inline bool overlaps_rows(Span v, const void* p, uint64_t rows, uint64_
     return at < row * stride * esz + cols * esz || (row + 1 < rows && v.hi - all.lo > (row + 1) * stride * esz);
 }
 
+// Whether two matrices of `rows` rows share a byte.  With the same stride in bytes they may lie beside each other, column
+// by column, in one buffer: row j of q then starts `in` bytes into row j + k of p's.  With other strides their extents decide.
+struct RowBytes {
+    const void* p;
+    uint64_t row, stride;     // bytes
+};
+__host__ inline bool rows_overlap(RowBytes p, RowBytes q, uint64_t rows) {
+    if (!rows || !p.row || !q.row) return false;
+    if (p.stride != q.stride || rows == 1) return overlap(span_of(p.p, rows, p.row, p.stride, 1), span_of(q.p, rows, q.row, q.stride, 1));
+    const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(q.p) - reinterpret_cast<uintptr_t>(p.p)), s = (int64_t)p.stride, n = (int64_t)rows;
+    const int64_t k = d >= 0 ? d / s : -((-d + s - 1) / s), in = d - k * s;
+    return (k > -n && k < n && (uint64_t)in < p.row) || (k + 1 > -n && k + 1 < n && (uint64_t)in + q.row > p.stride);
+}
+
 // vectors of 4-byte values (null: none), each aligned to them
 __host__ inline bool words_aligned(std::initializer_list<const void*> vectors) {
     for (const void* p : vectors)

@@ -74,3 +74,29 @@ def test_norm_gradients_that_write_over_what_they_read_are_refused(pkg):
     refuse(pkg, "overlap", backward, dw=ws + need - 4)
     taken(pkg, backward, dw=ws + need)
     taken(pkg, backward, dw=None, ws=dx)              # without dweight there is no workspace
+
+
+def test_matrices_beside_each_other_in_one_buffer(pkg):
+    """dx beside dy, codes beside values: rows of one buffer, each with its part of them."""
+    x, scales, w, dw, ws = places(5)
+    need = pkg.act8_rmsnorm_grad_workspace(5, 16)
+
+    def backward(dx, dres=None):
+        pkg.act8_rmsnorm_grad(x + ROOM // 2, scales, 5, 16, w, pkg.F32, 1e-6, x, pkg.F16, dx, dw, ws, need, dres, dy_stride=64, dresidual_stride=64,
+                              dx_stride=64)
+
+    def store(codes):
+        pkg.act8_store(x, pkg.F16, 5, 16, codes, scales, 64, 128)
+
+    for shift in range(-6 * 128, 6 * 128 + 1, 2):
+        meets = any(abs(shift + 128 * k) < 32 for k in range(-4, 5))
+        if shift and meets:
+            refuse(pkg, "overlap", backward, x + shift)
+            refuse(pkg, "overlap", backward, x + 64 * 128, x + 64 * 128 + shift)
+        else:
+            taken(pkg, backward, x + shift)
+            taken(pkg, backward, x + 64 * 128, x + 64 * 128 + shift)
+        if any(-16 < shift + 128 * k < 32 for k in range(-4, 5)):
+            refuse(pkg, "overlap", store, x + shift)
+        else:
+            taken(pkg, store, x + shift)

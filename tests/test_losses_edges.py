@@ -98,3 +98,23 @@ def test_preference_losses_that_write_over_what_they_read_are_refused(pkg):
         refuse(pkg, "overlap", call, rewards=at)
     for at in (coef, coef + 144):
         refuse(pkg, "overlap", call, stat=at)
+
+
+def brute(p, p_row, q, q_row, stride, rows):
+    """Whether two matrices share a byte, row by row."""
+    return any(p + i * stride < q + j * stride + q_row and q + j * stride < p + i * stride + p_row for i in range(rows) for j in range(rows))
+
+
+def test_a_gradient_beside_its_logits_in_one_buffer(pkg):
+    """Every place of a gradient around logits of the same stride: refused where a row of one meets a row of the other,
+    taken elsewhere (in the same place: in place)."""
+    z, y, lse, coef = places(4)
+    rows, vocab, stride = 4, 6, 20                    # FP16
+    for shift in range(-5 * stride, 5 * stride + 1):
+        def call():
+            pkg.token_logprob_grad(z, pkg.F16, rows, vocab, y, lse, coef, z + 2 * shift, row_stride=stride, grad_stride=stride)
+
+        if shift and brute(z, 12, z + 2 * shift, 12, 40, rows):
+            refuse(pkg, "overlap", call)
+        else:
+            taken(pkg, call)
