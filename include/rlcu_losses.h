@@ -41,11 +41,19 @@ int rlcu_token_logprob(const void* logits, uint32_t dtype, uint64_t rows, uint64
                        float inv_temperature, const int32_t* targets, float* logp, float* lse, void* stream);
 /* grad[t][j] = coef[t] * S * inv_temperature * ([j == targets[t]] - softmax_j), with coef[t] = dLoss/dlogp[t]
  * (coef = -1/tokens: the SFT loss of RL.cu) and S the loss scale; `lse` is what rlcu_token_logprob wrote for the
- * same logits; a row whose |lse| is above 2^24, which FP32 holds too coarsely for a probability, has a gradient of NaN.
- * A row with coef 0 takes no part. */
+ * same logits.  A row with coef 0 takes no part.
+ * FP32 holds lse to 2^-24 of itself, so probabilities taken from it are off by up to 2^-23 |lse| of themselves, and 1 - p
+ * of the target by that much in absolute terms: with logits around 1e4, 1e-3, more than a confident target has.  A row
+ * whose |lse| is above 2^24 has a gradient of NaN. */
 int rlcu_token_logprob_grad(const void* logits, uint32_t dtype, uint64_t rows, uint64_t vocab, uint64_t row_stride,
                             float inv_temperature, const int32_t* targets, const float* lse, const float* coef,
                             const rlcu_scaler_state* scaler, void* grad, uint64_t grad_stride, void* stream);
+/* The same with the log-probabilities that rlcu_token_logprob wrote beside lse (NULL: without): the target's 1 - p is
+ * taken from them, right to a few 2^-24 of itself whatever lse. */
+int rlcu_token_logprob_grad_logp(const void* logits, uint32_t dtype, uint64_t rows, uint64_t vocab, uint64_t row_stride,
+                                 float inv_temperature, const int32_t* targets, const float* lse, const float* logp,
+                                 const float* coef, const rlcu_scaler_state* scaler, void* grad, uint64_t grad_stride,
+                                 void* stream);
 
 /* -------- clipped policy loss --------------------------------------------- */
 /* estimator of KL(policy || reference) per token, d = logp - ref_logp */

@@ -44,7 +44,8 @@ EXPORTS = [
     "rlcu_zero1_make_plan", "rlcu_zero1_plan_pieces", "rlcu_zero1_unique_id", "rlcu_zero1_create",
     "rlcu_zero1_step", "rlcu_zero1_poll_error", "rlcu_zero1_check", "rlcu_zero1_destroy",
     "rlcu_checkpoint_save", "rlcu_checkpoint_peek", "rlcu_checkpoint_load",
-    "rlcu_token_logprob", "rlcu_token_logprob_grad", "rlcu_policy_loss", "rlcu_policy_loss_logp", "rlcu_preference_loss",
+    "rlcu_token_logprob", "rlcu_token_logprob_grad", "rlcu_token_logprob_grad_logp", "rlcu_policy_loss", "rlcu_policy_loss_logp",
+    "rlcu_preference_loss",
     "rlcu_losses_check", "rlcu_losses_selftest_wait", "rlcu_losses_selftest_tries",
     "rlcu_act8_blocks", "rlcu_act8_store", "rlcu_act8_load", "rlcu_act8_rmsnorm", "rlcu_act8_rmsnorm_grad_workspace",
     "rlcu_act8_rmsnorm_grad",
@@ -204,6 +205,7 @@ def lib() -> C.CDLL:
     logits = [vp, u32, u64, u64, u64, f, vp]          # data, dtype, rows, vocab, row stride, inv_temperature, targets
     L.rlcu_token_logprob.argtypes = logits + [vp, vp, vp]
     L.rlcu_token_logprob_grad.argtypes = logits + [vp, vp, vp, vp, u64, vp]
+    L.rlcu_token_logprob_grad_logp.argtypes = logits + [vp, vp, vp, vp, vp, u64, vp]
     L.rlcu_policy_loss.argtypes = logits + [vp, vp, vp, vp, vp, vp, vp, vp, u64, vp, u32, vp]
     L.rlcu_policy_loss_logp.argtypes = [vp, u64, vp, vp, vp, vp, vp, vp, vp, u32, vp]
     L.rlcu_preference_loss.argtypes = [vp, u64, vp, vp, vp, u64, vp, vp, vp, vp, vp, u32, vp]
@@ -430,10 +432,11 @@ def token_logprob(logits_ptr, dtype, rows, vocab, targets_ptr, logp_ptr, lse=Non
 
 
 def token_logprob_grad(logits_ptr, dtype, rows, vocab, targets_ptr, lse_ptr, coef_ptr, grad_ptr, row_stride=0,
-                       grad_stride=0, inv_temperature=1.0, scaler=None, stream=None):
-    """Gradient of the logits for ``coef`` = dloss/dlogp, times the loss scale of ``scaler``."""
-    check(lib().rlcu_token_logprob_grad(logits_ptr, dtype, rows, vocab, row_stride, inv_temperature, targets_ptr, lse_ptr,
-                                        coef_ptr, scaler, grad_ptr, grad_stride, stream))
+                       grad_stride=0, inv_temperature=1.0, scaler=None, stream=None, logp=None):
+    """Gradient of the logits for ``coef`` = dloss/dlogp, times the loss scale of ``scaler``.  With the forward call's
+    ``logp`` the target's entry is right to FP32 whatever the size of ``lse``."""
+    check(lib().rlcu_token_logprob_grad_logp(logits_ptr, dtype, rows, vocab, row_stride, inv_temperature, targets_ptr, lse_ptr,
+                                             logp, coef_ptr, scaler, grad_ptr, grad_stride, stream))
 
 
 def policy_hparams(clip_low=0.2, clip_high=0.2, dual_clip=0.0, kl_coef=0.0, kl_kind=KL_K3) -> PolicyHParams:

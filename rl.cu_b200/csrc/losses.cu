@@ -334,7 +334,7 @@ __device__ __forceinline__ void zero_row(void* grad, uint64_t at, uint32_t vocab
 // sixteen CTAs' registers.  4096 x 151936 bf16 takes 627 us this way.
 template <uint32_t DT, int MODE>
 __global__ void __launch_bounds__(kRowThreads)
-logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* coef_in) {
+logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* logp_in, const float* coef_in) {
     using E = Elem<DT>;
     using T = typename E::T;
     __shared__ float2 warp_part[kRowThreads / 32];
@@ -395,7 +395,7 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
             const bool empty = lse == -INFINITY;
             e = empty ? 0.0f : rintf(lse * kLog2E);
             kn = empty ? 0.0f * k : -k * exp2f(-fmaf(lse, kLog2E, -e));
-            ky = empty ? k : -k * expm1f(fmaf(E::up(x[y]), a.inv_temperature, -lse));
+            ky = empty ? k : -k * expm1f(logp_in ? logp_in[row] + 0.0f * lse : fmaf(E::up(x[y]), a.inv_temperature, -lse));
         }
         if (MODE == kModeGrad) __syncthreads();          // x[y] is read before it is overwritten in place
         T* g = static_cast<T*>(a.grad) + row * a.grad_stride;
@@ -768,7 +768,7 @@ constexpr int kGradThreads = 256, kGradPer = 4, kGradGroups = kGradThreads * kGr
 
 template <uint32_t DT>
 __global__ void __launch_bounds__(kGradThreads)
-logits_grad_kernel(LogitsArgs a, const float* lse_in, const float* coef_in, uint32_t runs) {
+logits_grad_kernel(LogitsArgs a, const float* lse_in, const float* logp_in, const float* coef_in, uint32_t runs) {
     using E = Elem<DT>;
     using T = typename E::T;
     const uint32_t row = blockIdx.x / runs, run = blockIdx.x - row * runs;
@@ -799,12 +799,13 @@ logits_grad_kernel(LogitsArgs a, const float* lse_in, const float* coef_in, uint
     // 2^(c z - log2e lse) = 2^(c z - e) * 2^(e - log2e lse), e an integer
     const bool empty = lse == -INFINITY;
     const float e = empty ? 0.0f : rintf(lse * kLog2E), kn = empty ? 0.0f * k : -k * exp2f(-fmaf(lse, kLog2E, -e));
-    // the target's logit is read by the thread that overwrites it
+    // the target's logit is read by the thread that overwrites it.  1 - p of a confident target comes from its
+    // log-probability where that is given: lse has lost those digits.  (A NaN lse is one of the whole row.)
     const uint32_t group = ((uint32_t)y - cut.head) / E::kVec;
     const bool in_groups = (uint32_t)y >= cut.head && (uint32_t)y < tail;
     const bool owns_y = in_groups ? group / kGradGroups == run && group % kGradThreads == tid : has_end && end_at == (uint32_t)y;
     float ky = 0.0f;
-    if (owns_y) ky = empty ? k : -k * expm1f(fmaf(E::up(x[y]), a.inv_temperature, -lse));
+    if (owns_y) ky = empty ? k : -k * expm1f(logp_in ? logp_in[row] + 0.0f * lse : fmaf(E::up(x[y]), a.inv_temperature, -lse));
     if (has_end) g[end_at] = E::down(kn * exp2_fast(fmaf(E::up(x[end_at]), c, -e)));
 #pragma unroll
     for (int j = 0; j < kGradPer; j++)
@@ -1248,14 +1249,14 @@ int sm_count(int* out) {
 }
 
 template <int MODE>
-int launch_rows(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, const float* lse, const float* coef, cudaStream_t s) {
+int launch_rows(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, const float* lse, const float* logp, const float* coef, cudaStream_t s) {
     int sms = 0;
     if (const int rc = sm_count(&sms)) return rc;
     const uint64_t most = (uint64_t)sms * 4;
     const int grid = (int)(a.rows < most ? a.rows : most);
-    if (dtype == RLCU_F16) logits_row_kernel<RLCU_F16, MODE><<<grid, kRowThreads, 0, s>>>(a, p, lse, coef);
-    else if (dtype == RLCU_BF16) logits_row_kernel<RLCU_BF16, MODE><<<grid, kRowThreads, 0, s>>>(a, p, lse, coef);
-    else logits_row_kernel<RLCU_F32, MODE><<<grid, kRowThreads, 0, s>>>(a, p, lse, coef);
+    if (dtype == RLCU_F16) logits_row_kernel<RLCU_F16, MODE><<<grid, kRowThreads, 0, s>>>(a, p, lse, logp, coef);
+    else if (dtype == RLCU_BF16) logits_row_kernel<RLCU_BF16, MODE><<<grid, kRowThreads, 0, s>>>(a, p, lse, logp, coef);
+    else logits_row_kernel<RLCU_F32, MODE><<<grid, kRowThreads, 0, s>>>(a, p, lse, logp, coef);
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
 }
@@ -1329,20 +1330,20 @@ int launch_logits(const LogitsArgs& a, const PolicyArgs& p, uint32_t dtype, cuda
     const uint64_t groups = a.vocab / (16 / esz);
     const bool fits = MODE != kModePolicy || groups <= (uint64_t)kMostCluster * kWide * kMostHeld;
     if ((MODE == kModePolicy && !alike(a, esz)) || !fits || groups < 64 || a.rows > 0x7FFFFFFFull / kMostCluster)
-        return launch_rows<MODE>(a, p, dtype, nullptr, nullptr, s);
+        return launch_rows<MODE>(a, p, dtype, nullptr, nullptr, nullptr, s);
     if (dtype == RLCU_F16) return launch_logits_dt<RLCU_F16, MODE>(a, p, sms, groups, s);
     if (dtype == RLCU_BF16) return launch_logits_dt<RLCU_BF16, MODE>(a, p, sms, groups, s);
     return launch_logits_dt<RLCU_F32, MODE>(a, p, sms, groups, s);
 }
 
-int launch_grad(const LogitsArgs& a, uint32_t dtype, const float* lse, const float* coef, cudaStream_t s) {
+int launch_grad(const LogitsArgs& a, uint32_t dtype, const float* lse, const float* logp, const float* coef, cudaStream_t s) {
     const size_t esz = dtype_bytes(dtype);
     const uint64_t groups = a.vocab / (16 / esz), runs = (groups + kGradGroups - 1) / kGradGroups;
-    if (!alike(a, esz) || groups < 64 || a.rows * runs > 0x7FFFFFFFull) return launch_rows<kModeGrad>(a, PolicyArgs{}, dtype, lse, coef, s);
+    if (!alike(a, esz) || groups < 64 || a.rows * runs > 0x7FFFFFFFull) return launch_rows<kModeGrad>(a, PolicyArgs{}, dtype, lse, logp, coef, s);
     const unsigned grid = (unsigned)(a.rows * runs);
-    if (dtype == RLCU_F16) logits_grad_kernel<RLCU_F16><<<grid, kGradThreads, 0, s>>>(a, lse, coef, (uint32_t)runs);
-    else if (dtype == RLCU_BF16) logits_grad_kernel<RLCU_BF16><<<grid, kGradThreads, 0, s>>>(a, lse, coef, (uint32_t)runs);
-    else logits_grad_kernel<RLCU_F32><<<grid, kGradThreads, 0, s>>>(a, lse, coef, (uint32_t)runs);
+    if (dtype == RLCU_F16) logits_grad_kernel<RLCU_F16><<<grid, kGradThreads, 0, s>>>(a, lse, logp, coef, (uint32_t)runs);
+    else if (dtype == RLCU_BF16) logits_grad_kernel<RLCU_BF16><<<grid, kGradThreads, 0, s>>>(a, lse, logp, coef, (uint32_t)runs);
+    else logits_grad_kernel<RLCU_F32><<<grid, kGradThreads, 0, s>>>(a, lse, logp, coef, (uint32_t)runs);
     RLCU_CUDA(cudaGetLastError());
     return RLCU_OK;
 }
@@ -1380,20 +1381,28 @@ extern "C" int rlcu_token_logprob(const void* logits, uint32_t dtype, uint64_t r
     return launch_logits<kModeLogprob>(a, PolicyArgs{}, dtype, (cudaStream_t)stream);
 }
 
+extern "C" int rlcu_token_logprob_grad_logp(const void* logits, uint32_t dtype, uint64_t rows, uint64_t vocab,
+                                            uint64_t row_stride, float inv_temperature, const int32_t* targets,
+                                            const float* lse, const float* logp, const float* coef,
+                                            const rlcu_scaler_state* scaler, void* grad, uint64_t grad_stride, void* stream) {
+    if (const int rc = check_logits(logits, dtype, rows, vocab, row_stride, inv_temperature, targets)) return rc;
+    if (const int rc = check_grad(logits, dtype, rows, vocab, row_stride, grad, grad_stride)) return rc;
+    if (rows && (!lse || !coef)) return set_error(RLCU_ERR_INVALID, "null lse or coef");
+    if (!words_aligned({targets, lse, logp, coef, scaler})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
+    if (!rows) return RLCU_OK;
+    for (const Span& in : {words(targets, rows), words(lse, rows), words(logp, rows), words(coef, rows), bytes_of(scaler, sizeof *scaler)})
+        if (overlaps_rows(in, grad, rows, vocab, grad_stride, dtype_bytes(dtype)))
+            return set_error(RLCU_ERR_INVALID, "gradient overlaps a vector that the call reads");
+    LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, nullptr, nullptr, grad, grad_stride, scaler, wait_tries};
+    return launch_grad(a, dtype, lse, logp, coef, (cudaStream_t)stream);
+}
+
 extern "C" int rlcu_token_logprob_grad(const void* logits, uint32_t dtype, uint64_t rows, uint64_t vocab,
                                        uint64_t row_stride, float inv_temperature, const int32_t* targets,
                                        const float* lse, const float* coef, const rlcu_scaler_state* scaler, void* grad,
                                        uint64_t grad_stride, void* stream) {
-    if (const int rc = check_logits(logits, dtype, rows, vocab, row_stride, inv_temperature, targets)) return rc;
-    if (const int rc = check_grad(logits, dtype, rows, vocab, row_stride, grad, grad_stride)) return rc;
-    if (rows && (!lse || !coef)) return set_error(RLCU_ERR_INVALID, "null lse or coef");
-    if (!words_aligned({targets, lse, coef, scaler})) return set_error(RLCU_ERR_INVALID, "%s", kUnaligned);
-    if (!rows) return RLCU_OK;
-    for (const Span& in : {words(targets, rows), words(lse, rows), words(coef, rows), bytes_of(scaler, sizeof *scaler)})
-        if (overlaps_rows(in, grad, rows, vocab, grad_stride, dtype_bytes(dtype)))
-            return set_error(RLCU_ERR_INVALID, "gradient overlaps a vector that the call reads");
-    LogitsArgs a = {logits, rows, row_stride, (uint32_t)vocab, inv_temperature, targets, nullptr, nullptr, grad, grad_stride, scaler, wait_tries};
-    return launch_grad(a, dtype, lse, coef, (cudaStream_t)stream);
+    return rlcu_token_logprob_grad_logp(logits, dtype, rows, vocab, row_stride, inv_temperature, targets, lse, nullptr, coef, scaler, grad,
+                                        grad_stride, stream);
 }
 
 extern "C" int rlcu_policy_loss_logp(const float* logp, uint64_t tokens, const float* old_logp, const float* ref_logp,

@@ -118,3 +118,16 @@ def test_a_gradient_beside_its_logits_in_one_buffer(pkg):
             refuse(pkg, "overlap", call)
         else:
             taken(pkg, call)
+
+
+def test_log_probabilities_given_to_the_gradient_are_checked(pkg):
+    z, y, lse, coef, g, logp = places(6)
+
+    def call(logp):
+        pkg.token_logprob_grad(z, pkg.F16, 3, 16, y, lse, coef, g, logp=logp)
+
+    refuse(pkg, "aligned", call, logp + 2)
+    for at in (g, g + 92, g - 8):
+        refuse(pkg, "overlap", call, at)
+    taken(pkg, call, logp)
+    taken(pkg, call, None)
