@@ -993,7 +993,8 @@ __device__ __forceinline__ void preference_term(const rlcu_preference_hparams& h
     if (hp.kind == RLCU_PREF_SIGMOID) {
         const double e = hp.label_smoothing, tail = log1p(exp(-fabs(h)));
         // -log sigmoid(h) = max(-h, 0) + log(1 + exp(-|h|))
-        loss = (1.0 - e) * (fmax(-h, 0.0) + tail) + e * (fmax(h, 0.0) + tail);
+        loss = (1.0 - e) * (fmax(-h, 0.0) + tail);
+        if (e > 0.0) loss += e * (fmax(h, 0.0) + tail);                // (not 0 times an infinite h)
         slope = e / (1.0 + exp(-h)) - (1.0 - e) / (1.0 + exp(h));
     } else if (hp.kind == RLCU_PREF_HINGE) {
         loss = fmax(0.0, 1.0 - h);

@@ -51,3 +51,22 @@ def test_preference_records_of_clusters_with_idle_ctas(pkg, pairs, tokens):
     s = stat_of(pkg.PreferenceStat, records[0])
     assert (s.pairs, s.correct) == (pairs, int((sums[:, 0] > sums[:, 1]).sum()))
     assert abs(s.loss - loss) <= abs(loss) * 2.0 ** -20 and abs(s.margin - margin) <= abs(margin) * 2.0 ** -20
+
+
+@pytest.mark.parametrize("kind,smoothing", [(0, 0.0), (0, 0.1), (1, 0.0)])
+def test_preference_pairs_of_infinite_margin(pkg, kind, smoothing):
+    """A token the policy gives no probability (log p = -inf) in a rejected sequence settles its pair: loss 0 and gradient 0,
+    unless labels are smoothed; in a chosen one the loss is infinite and its slope the steepest."""
+    inf, e = float("inf"), float(torch.tensor(smoothing))
+    hp = pkg.preference_hparams(0.25, 0.0, smoothing, kind)
+    cases = (([-1.0, -2.0, -0.5, -inf], inf, inf if smoothing else 0.0, e, 1),
+             ([-2.5, -inf, -1.5, -1.0], -inf, inf, -(1 - e) if kind == 0 else -1.0, 0))
+    for logp, margin, loss, slope, correct in cases:
+        lp, ob = torch.tensor(logp).cuda(), torch.tensor([0, 2, 4], dtype=torch.int32).cuda()
+        coef, stat = torch.full((4,), 7.0, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+        pkg.preference_loss(lp.data_ptr(), 4, ob.data_ptr(), 1, hp, stat.data_ptr(), coef.data_ptr())
+        torch.cuda.synchronize()
+        s = stat_of(pkg.PreferenceStat, stat)
+        assert (s.loss, s.margin, s.correct) == (loss, margin, correct)
+        want = torch.tensor([0.25 * slope] * 2 + [-0.25 * slope] * 2)
+        assert (coef.cpu() - want).abs().max() <= 2.0 ** -26          # one rounding of a quarter
