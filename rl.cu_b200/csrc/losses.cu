@@ -62,9 +62,11 @@ struct PolicyTerm {
 // (a KL term given).
 __device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& p, float logp, float a, float w, float old, float ref) {
     PolicyTerm o;
-    o.ratio = p.old_logp ? expf(logp - old) : 1.0f;
+    const float since = p.old_logp ? logp - old : 0.0f;
+    o.ratio = expf(since);
     const float lo = 1.0f - p.hp.clip_low, hi = 1.0f + p.hp.clip_high;
-    const float kept = o.ratio * a;
+    // (a ratio beyond FP32 is still a number, and nothing of it is left where there is no advantage)
+    const float kept = a == 0.0f && o.ratio == INFINITY && since < INFINITY ? 0.0f : o.ratio * a;
     float best = kept, slope = kept;
     // a comparison with NaN is false: a NaN ratio stays in `best`, `slope` and so in the gradient
     const float held = (o.ratio < lo ? lo : (o.ratio > hi ? hi : o.ratio)) * a;
