@@ -43,7 +43,8 @@ int rlcu_act8_load(const uint8_t* codes, uint64_t code_stride, const uint8_t* sc
                    void* x, uint32_t dtype, uint64_t x_stride, void* stream);
 
 /* The norm again: y = x * rstd * weight with rstd = 1 / sqrt(mean(x^2) + eps) per row, x the checkpoint's values.
- * weight has `cols` values of weight_dtype (RL.cu: F32); rstd may be NULL. */
+ * weight has `cols` values of weight_dtype (RL.cu: F32); rstd may be NULL.  Squares are summed in FP32: a row whose sum is
+ * beyond it (values above 1e18 or so) has rstd = 0. */
 int rlcu_act8_rmsnorm(const uint8_t* codes, uint64_t code_stride, const uint8_t* scales, uint64_t rows, uint64_t cols,
                       const void* weight, uint32_t weight_dtype, float eps, void* y, uint32_t dtype, uint64_t y_stride,
                       float* rstd, void* stream);

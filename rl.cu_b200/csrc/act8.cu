@@ -423,7 +423,8 @@ __device__ __forceinline__ float2 block_sum2(float x, float y, float2* smem) {
     return make_float2(x, y);
 }
 
-// One CTA per row at a time, the row decoded twice: rows wider than the kernels below hold.
+// One CTA per row at a time, the row decoded twice, a code per access: rows wider than the kernels below hold.  Not fast:
+// 4096 x 16384 bf16 154 us, its gradient (whose partial sums are in memory) 1231 us; the bytes alone would take 31 and 72.
 template <uint32_t DT>
 __global__ void __launch_bounds__(kAct8Threads)
 norm_kernel(NormArgs a) {
@@ -542,7 +543,7 @@ __device__ __forceinline__ void load_weights(const NormArgs& a, uint32_t col, in
 
 // A thread's 16 columns lie in one block, so their scale s comes out of the sums: sum x^2 = s^2 sum c^2 and so on, with
 // c the codes, and x itself is never formed.  Bound by HBM and, a row at a time, by the latency of its sum: 16384 x 4096
-// bf16 39 us, 0.79 of the copy rate (one row per barrier 43 us, scalar arithmetic 54 us).
+// bf16 39 to 41 us on different GPUs, 0.79 to 0.75 of the copy rate (one row per barrier 43 us, scalar arithmetic 54 us).
 template <uint32_t DT, int TPR, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 norm_vec_kernel(NormArgs a, uint32_t rows_per_cta) {
@@ -676,9 +677,11 @@ struct GradRow {
 };
 
 // The gradient: rows are dealt to the CTAs in a fixed order, so that dweight's partial sums are the same in every run;
-// the next row is on its way in registers.  16384 x 4096 bf16 with a residual: 86 us with the second kernel, 0.83 of the
-// copy rate.  Issue slots were 69 % busy with scalar arithmetic (95 us); packed pairs and the scale taken out of the sums
-// left 86 us.  More CTAs per SM spill (177 to 255 us); the next row by cp.async is slower (112 us).
+// the next row is on its way in registers.  16384 x 4096 bf16 with a residual: 86 to 91 us on different GPUs with the
+// second kernel, 0.83 to 0.79 of the copy rate; f32, without the row ahead, 160 us, 0.83.  Issue slots were 69 % busy with
+// scalar arithmetic (95 us); packed pairs and the scale taken out of the sums left 86 us.  More CTAs per SM spill (177 to 255
+// us); the next row by cp.async is slower (112 us).  With 512 threads a row (more than 4096 columns) a thread keeps 8 to 24
+// bytes in local memory as it is.
 template <uint32_t DT, int TPR, int THREADS>
 __global__ void __launch_bounds__(THREADS, 512 / THREADS)
 norm_grad_vec_kernel(NormArgs a) {
@@ -931,8 +934,8 @@ norm_grad_col_kernel(NormArgs a) {
     if (a.dweight) add_parts_in_cluster(a);
 }
 
-// dweight from the CTAs' partial sums: a CTA per 32 columns, each warp every 32nd part, then the warps in order.  Launched
-// while the gradient kernel still runs; it waits for its end.
+// dweight from the CTAs' partial sums: a CTA per 32 columns, each warp every 32nd part, then the warps in order.  Its
+// launch is prepared while the gradient kernel still runs; it starts when that one's last CTA has left.
 constexpr int kWeightThreads = 1024;
 
 __global__ void __launch_bounds__(kWeightThreads)

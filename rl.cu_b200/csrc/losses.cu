@@ -340,7 +340,7 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
     using E = Elem<DT>;
     using T = typename E::T;
     __shared__ float2 warp_part[kRowThreads / 32];
-    __shared__ float4 answer;                         // e, -k / s, k (1 - p_y), factor of z (policy kernel: 0 for a row to be looked at again)
+    __shared__ float4 answer;                         // e, -k / s, k (1 - p_y), factor of z
     const float c = a.inv_temperature * kLog2E;
     const float S = a.scaler ? a.scaler->scale : 1.0f;
 
@@ -368,9 +368,10 @@ logits_row_kernel(LogitsArgs a, PolicyArgs p, const float* lse_in, const float* 
             for (uint32_t i = tail + threadIdx.x; i < a.vocab; i += kRowThreads) o.add(E::up(x[i]), c);
             o = add_in_block(o, warp_part, c);
             if (threadIdx.x < 32) {
+                const float z_y = E::up(x[y]);
                 RowAnswer r;
-                if (o.says_nothing()) r = row_answer(top_by_warp<DT>(x, a.vocab), E::up(x[y]), c, a.inv_temperature);
-                else r = row_answer<false>(o, E::up(x[y]), c);
+                if (__any_sync(0xFFFFFFFFu, o.says_nothing())) r = row_answer(top_by_warp<DT>(x, a.vocab), z_y, c, a.inv_temperature);
+                else r = row_answer<false>(o, z_y, c);
                 if (threadIdx.x == 0) {
                     a.logp[row] = r.logp;
                     if (a.lse) a.lse[row] = r.lse;
@@ -597,12 +598,13 @@ struct RowFeed {
 // and keeps it in registers between the sum and the gradient: the logits are read once, the gradient is written once.
 // Several clusters share an SM (four CTAs of 256 threads with up to ten groups each: 160 KB of its registers), so that
 // one row's loads and stores run under another's arithmetic.
-// Measured (B200, a tenth of the rows without part): 4096 x 151936 bf16 457 us, 0.79 of the copy rate (6.55 TB/s) for the
-// bytes it cannot do without; 1000 x 151936 f32 229 us, 0.81.  A row takes a CTA about 14,500 cycles: 3,500 until its loads
-// are there, 3,000 for the sum, 3,000 to 4,500 to exchange it, 1,100 for the row's factors, 2,000 for the gradient; with
-// four CTAs per SM the special-function units and the issue slots are each a little over half busy.  The same kernel
-// without any arithmetic takes 421 us, a plain copy of the same bytes 335 us.  Fetching the next row ahead (into L2, into
-// shared memory by cp.async or by a bulk copy), a second row in the same loop, and five or six CTAs per SM with part of
+// Measured (B200, a tenth of the rows without part): 4096 x 151936 bf16 457 to 469 us on different GPUs, 0.79 to 0.77 of the
+// copy rate (6.55 TB/s) for the bytes it cannot do without; 1000 x 151936 f32, all with part, 217 to 223 us, 0.86 to 0.83.
+// (With ten groups of a 16-bit type a thread keeps 8 bytes in local memory.)  A row takes a CTA about 14,500 cycles: 3,500
+// until its loads are there, 3,000 for the sum, 3,000 to 4,500 to exchange it, 1,100 for the row's factors, 2,000 for the
+// gradient; with four CTAs per SM the special-function units and the issue slots are each a little over half busy.  The same
+// kernel without any arithmetic takes 421 us, a plain copy of the same bytes 335 us.  Fetching the next row ahead (into L2,
+// into shared memory by cp.async or by a bulk copy), a second row in the same loop, and five or six CTAs per SM with part of
 // the row in shared memory were all slower (453 to 720 us; L2 prefetch gained 2 % here and lost 20 % for f32).
 template <uint32_t DT, int THREADS, int NV>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
@@ -612,7 +614,7 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
     __shared__ ClusterSum<THREADS / 32> sums;
     __shared__ RowFeed feed;
     __shared__ float inputs[8];
-    __shared__ float4 answer;                         // e, -k / s, k (1 - p_y), factor of z (policy kernel: 0 for a row to be looked at again)
+    __shared__ float4 answer;                         // e, -k / s, k (1 - p_y), 0 for a row to be looked at again
     const uint32_t C = cooperative_groups::this_cluster().num_blocks(), rank = cooperative_groups::this_cluster().block_rank();
     const int tid = threadIdx.x;
     const bool asks = rank == 0 && tid == 0;
@@ -700,8 +702,8 @@ logits_policy_kernel(LogitsArgs a, PolicyArgs p) {
 }
 
 // Log-probabilities alone: a cluster (one CTA, unless rows are few) per row, kDepth groups per thread on their way in
-// registers.  Bound by HBM: 2048 x 151936 bf16 97 us, 0.88 of the copy rate; the same with the groups on their way by
-// cp.async through shared memory 106 us, with CTAs that stay and take over rows 110 us.
+// registers.  Bound by HBM: 2048 x 151936 bf16 95 to 102 us on different GPUs, 0.90 to 0.84 of the copy rate; on one of them
+// 97, with the groups on their way by cp.async through shared memory 106, with CTAs that stay and take over rows 110.
 constexpr int kDepth = 5;
 
 template <uint32_t DT, int THREADS>
@@ -752,7 +754,7 @@ logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
         o = sums.template take<Online>(c, 0, C, a.tries);
         if (rank == 0) {
             RowAnswer r;
-            if (__shfl_sync(0xFFFFFFFFu, o.says_nothing(), 0)) r = row_answer(top_by_warp<DT>(now.x, a.vocab), z_y, c, a.inv_temperature);
+            if (__any_sync(0xFFFFFFFFu, o.says_nothing())) r = row_answer(top_by_warp<DT>(now.x, a.vocab), z_y, c, a.inv_temperature);
             else r = row_answer<false>(o, z_y, c);
             if (tid == 0) {
                 a.logp[row] = r.logp;
@@ -764,8 +766,8 @@ logits_sum_kernel(LogitsArgs a, PolicyArgs p) {
 }
 
 // The gradient alone (the sum is known): elementwise, a CTA per run of kGradGroups groups of a row, so that the grid
-// moves through memory in order.  Bound by HBM: with the sum before it, 1000 x 50001 f32 97 us for 560 MB (the logits
-// are read twice), 0.88 of the copy rate.
+// moves through memory in order.  Bound by HBM: with the sum before it, 1000 x 50001 f32 95 to 97 us for 560 MB (the logits
+// are read twice), 0.90 to 0.88 of the copy rate.
 constexpr int kGradThreads = 256, kGradPer = 4, kGradGroups = kGradThreads * kGradPer;
 
 template <uint32_t DT>
@@ -891,7 +893,8 @@ __device__ __forceinline__ void spoil(const LogitsArgs& a, uint32_t dtype, uint6
 // Weighted sums of the policy loss over all tokens, and the gradient by log-probability.  `a` (with targets): tokens whose
 // target is out of range take no part; rows marked by logits_policy_kernel are done first; and after a wait of that kernel
 // has given up, when rows may have been left out, nothing of the call is left that looks like a result.  One cluster: its
-// CTAs hand their sums to the first one, so the record needs no scratch memory and no second launch.  Bound by latency: 16384 tokens 4.8 us in a graph.
+// CTAs hand their sums to the first one, so the record needs no scratch memory and no second launch.  Bound by latency:
+// 16384 tokens 4.7 us in a graph.
 __global__ void __launch_bounds__(kVectorThreads)
 policy_kernel(const float* logp, uint64_t tokens, const __grid_constant__ LogitsArgs a, uint32_t dtype,
               const __grid_constant__ PolicyArgs p, float* coef, rlcu_policy_stat* stat, uint32_t flags) {
@@ -931,12 +934,13 @@ sums:
             if (threadIdx.x == 0) warps[0].l = warps[0].w = NAN;
             __syncthreads();
         } else {
-            for (uint64_t t = rank * kVectorThreads; t < tokens; t += t % kVectorThreads == kVectorThreads - 1 ? (C - 1) * kVectorThreads + 1 : 1) {
-                if (__float_as_uint(logp[t]) != kLookAgain) continue;   // (one thread changes it, behind a barrier all pass)
-                if (dtype == RLCU_F16) look_again<RLCU_F16>(a, p, t);
-                else if (dtype == RLCU_BF16) look_again<RLCU_BF16>(a, p, t);
-                else look_again<RLCU_F32>(a, p, t);
-            }
+            for (uint64_t base = rank * kVectorThreads; base < tokens; base += C * kVectorThreads)
+                for (uint64_t t = base; t < tokens && t < base + kVectorThreads; t++) {
+                    if (__float_as_uint(logp[t]) != kLookAgain) continue;       // (one thread changes it, behind a barrier)
+                    if (dtype == RLCU_F16) look_again<RLCU_F16>(a, p, t);
+                    else if (dtype == RLCU_BF16) look_again<RLCU_BF16>(a, p, t);
+                    else look_again<RLCU_F32>(a, p, t);
+                }
             goto sums;
         }
     }
@@ -1012,8 +1016,9 @@ __device__ __forceinline__ void preference_term(const rlcu_preference_hparams& h
 
 // One cluster, so that the record needs no scratch memory and no second launch.  CTA r has the pairs r, r + C, ... and
 // works on kBatch of them at a time, whatever their lengths: their tokens are cut into at most kSegments segments of
-// equal length, a warp sums a segment, and the segments of a sequence are added in order.  Bound by latency and by what 16
-// SMs read: 128 pairs of 2048 tokens 16 us (a CTA per pair in turn: 706 us), one pair of 200 6 us in a graph.
+// equal length, a warp sums a segment, and the segments of a sequence are added in order.  Bound by latency, that of
+// loads of 4 bytes a lane and of five barriers of 1024 threads per batch: 128 pairs of 2048 tokens 16 us (a CTA per pair in
+// turn: 706 us; 16 SMs could read them in 2 to 3), one pair of 200 7 us in a graph.
 constexpr int kBatch = 16, kSegments = 512;
 
 __global__ void __launch_bounds__(kVectorThreads)
@@ -1351,7 +1356,8 @@ int launch_grad(const LogitsArgs& a, uint32_t dtype, const float* lse, const flo
     return RLCU_OK;
 }
 
-// behind: launched while the call's own kernel before it still runs (policy_kernel waits for its end)
+// behind: its launch is prepared while the call's own kernel before it still runs; it starts when that one's last CTA has
+// left, since none of them triggers it sooner, and waits for what they wrote
 int launch_policy(const float* logp, uint64_t tokens, const LogitsArgs& a, uint32_t dtype, const PolicyArgs& p, float* coef,
                   rlcu_policy_stat* stat, uint32_t flags, bool behind, cudaStream_t s) {
     cudaLaunchAttribute attr[2];

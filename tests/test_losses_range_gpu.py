@@ -155,3 +155,51 @@ def test_rows_of_nothing_but_absent_logits(pkg, it, vocab):
     rest[torch.arange(4), y.long()] = False
     for t, at_target in ((grad, it), (fused, -it)):
         assert bool((t[rest] == 0).all()) and bool((t[~rest] == torch.tensor(at_target)).all())
+
+
+def test_rows_looked_at_again_in_graphs_and_on_two_streams(pkg):
+    """A third of the rows are nothing but one mask; the calls are captured on two streams, replayed together on other
+    contents, and give what calls one after the other give."""
+    rows, vocab = 1100, 4096
+    sets = []
+    for k in range(2):
+        z = torch.empty(rows, vocab, dtype=torch.bfloat16, device="cuda")
+        y = torch.randint(0, vocab, (rows,), generator=torch.Generator().manual_seed(k), dtype=torch.int32).cuda()
+        one = torch.ones(rows, device="cuda")
+        sets.append((z, y, one, torch.empty(rows, device="cuda"), torch.empty_like(z), torch.zeros(8, dtype=torch.int32, device="cuda")))
+    hp = pkg.policy_hparams()
+
+    def fill(seed):
+        for k, s in enumerate(sets):
+            s[0].copy_(gaussian(rows, vocab, "bf16", seed + 10 * k))
+            s[0][k::3] = -1e12
+            s[0][k + 1, 7:] = -1e20
+
+    def call(s, stream):
+        z, y, one, logp, grad, stat = s
+        pkg.policy_loss(z.data_ptr(), pkg.BF16, rows, vocab, y.data_ptr(), one.data_ptr(), one.data_ptr(), hp, logp.data_ptr(), grad.data_ptr(),
+                        stat.data_ptr(), stream=stream)
+
+    fill(0)
+    graphs, streams = [], [torch.cuda.Stream() for _ in sets]
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(s, torch.cuda.current_stream().cuda_stream)
+    fill(1)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                g.replay()
+    torch.cuda.synchronize()
+    kept = [[t.clone() for t in s[3:]] for s in sets]
+    for s, old in zip(sets, kept):
+        for t in s[3:]:
+            t.zero_()
+        call(s, None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(old, s[3:]))
+    for k, (logp, grad, _) in enumerate(kept):
+        assert ((logp[k::3].double() + math.log(vocab)).abs() <= 2.0 ** -17).all() and bool(torch.isfinite(grad).all())
+    pkg.losses_check()
