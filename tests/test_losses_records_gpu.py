@@ -9,7 +9,7 @@ from test_losses_gpu import check_preference, off_the_borders, stat_of
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("tokens", [1025, 1500, 2048, 3072, 4097, 9000])
+@pytest.mark.parametrize("tokens", [1025, 1500, 2048, 3000, 4097, 9000])
 def test_policy_records_of_clusters_with_idle_ctas(pkg, tokens):
     g = torch.Generator().manual_seed(tokens)
     logp = -torch.rand(tokens, generator=g) * 3
