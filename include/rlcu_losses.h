@@ -143,7 +143,7 @@ typedef struct rlcu_preference_stat {
  * in the mask.
  *   ref_logp    : NULL: without a reference
  *   mask        : one byte per token, 0 takes no part (NULL: all do); what a masked place holds does not matter
- *   pair_weight : NULL: 1/pairs each
+ *   pair_weight : NULL: 1/pairs each.  A pair of weight 0 has no loss, no margin and a coef of 0, whatever its tokens hold
  *   coef        : dloss/dlogp, 0 for masked tokens and for tokens of no sequence; may be NULL, and may be the buffer of logp
  *   rewards     : beta * s of each sequence; may be NULL
  * A sequence without tokens has s = 0. */

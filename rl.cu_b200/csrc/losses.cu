@@ -1119,12 +1119,14 @@ preference_kernel(PreferenceArgs a) {
             double h, loss, slope;
             preference_term(a.hp, s[0], s[1], h, loss, slope);
             const double w = a.pair_weight ? (double)a.pair_weight[pair] : 1.0 / (double)a.pairs;
-            loss_sum += w * loss;
-            margin_sum += w * h;
+            if (w != 0.0) {                           // (not 0 times an infinite margin or NaN)
+                loss_sum += w * loss;
+                margin_sum += w * h;
+            }
             correct += s[0] > s[1];
             for (int q = 0; q < 2; q++) {
                 if (a.rewards) a.rewards[2 * pair + q] = (float)((double)a.hp.beta * s[q]);
-                coefs[2 * tid + q] = (float)((q ? -slope : slope) * w * share[q]);
+                coefs[2 * tid + q] = w != 0.0 ? (float)((q ? -slope : slope) * w * share[q]) : 0.0f;
             }
         }
         __syncthreads();

@@ -70,3 +70,27 @@ def test_preference_pairs_of_infinite_margin(pkg, kind, smoothing):
         assert (s.loss, s.margin, s.correct) == (loss, margin, correct)
         want = torch.tensor([0.25 * slope] * 2 + [-0.25 * slope] * 2)
         assert (coef.cpu() - want).abs().max() <= 2.0 ** -26          # one rounding of a quarter
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_preference_pairs_of_weight_zero_hold_anything(pkg, kind):
+    """Pairs that pad a batch: the same record and coefficients as the batch without them, and 0 at their tokens."""
+    g = torch.Generator().manual_seed(kind)
+    logp = -torch.rand(60, generator=g)
+    w = torch.tensor([0.25, 0.0, 0.5, 0.0, 0.25])
+    offsets = torch.arange(11, dtype=torch.int32) * 6
+    bad = logp.clone()
+    bad[12:24] = float("nan")
+    bad[40] = -float("inf")
+    results = []
+    for lp, pairs in ((bad, [0, 1, 2, 3, 4]), (torch.cat([logp[0:12], logp[24:36], logp[48:60]]), [0, 2, 4])):
+        d = [lp.cuda(), offsets[:2 * len(pairs) + 1].cuda(), w[pairs].cuda()]
+        coef, stat = torch.full((lp.numel(),), 7.0, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+        pkg.preference_loss(d[0].data_ptr(), lp.numel(), d[1].data_ptr(), len(pairs), pkg.preference_hparams(0.3, kind=kind), stat.data_ptr(),
+                            coef.data_ptr(), pair_weight=d[2].data_ptr())
+        torch.cuda.synchronize()
+        results.append((coef.cpu(), stat_of(pkg.PreferenceStat, stat)))
+    (coef, s), (short, t) = results
+    assert (s.loss, s.margin, s.pairs, t.pairs) == (t.loss, t.margin, 5, 3)
+    assert bool((coef[12:24] == 0).all()) and bool((coef[36:48] == 0).all())
+    assert torch.equal(torch.cat([coef[0:12], coef[24:36], coef[48:60]]), short)
